@@ -236,6 +236,47 @@ int moe_block_forward_add_rms(const void* x, const void* h, const void* norm_wei
                               long long* top_k_index, void* top_k_weights, void* logits,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- 8-bit activations -------------------------------------------------------------------
+ * No counterpart in the reference, whose activations are bf16 throughout. A row in 8 bits is
+ * e4m3fn values with one fp32 scale s: amax / 448 over the row's finite values (amax counts as
+ * 2^-100 at least; 1 for a row of zeros), values e4m3(v / s), ties to even; NaN and infinite
+ * values become NaN. */
+
+/* q [T, n] e4m3 and scale [T] fp32 of x [T, n] bf16; n a multiple of 8 up to 8192. */
+int moe_quantize_rows(const void* x, int T, int n, void* q, float* scale, void* stream);
+
+/* moe_add_rmsnorm with the norm in 8 bits, made from its fp32 values: q [T, H], scale [T], and
+ * norm [T, H] bf16 unless null. total is written only when h is given. */
+int moe_add_rmsnorm_fp8(const void* x, const void* h, const void* weight, int T, int H, float eps,
+                        void* total, void* q, float* scale, void* norm, void* stream);
+
+/* out [M, N] = bf16(residual + mul * act(x_scale_m w_scale_n sum_k x[m, k] w[n, k] + bias_n)),
+ * fp32 in between. x [M, K] and w [N, K] are both bf16 (no scales, K a multiple of 8) or both
+ * e4m3 (MOE_WEIGHTS_FP8_E4M3, with x_scale [M] and w_scale [N], K a multiple of 16); rows are
+ * ldx / ldw elements apart and start at multiples of 16 bytes. bias [N] is bf16, or fp32 with
+ * bias_f32; mul and residual are [M, N] bf16. bias, mul and residual may be null. */
+#define MOE_ACT_NONE 0
+#define MOE_ACT_RELU 1
+#define MOE_ACT_SILU 2
+#define MOE_ACT_GELU 3
+#define MOE_ACT_GELU_TANH 4
+int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
+               const float* w_scale, int dtype, int M, int K, int N, const void* bias,
+               int bias_f32, int act, const void* mul, const void* residual, void* out,
+               void* stream);
+
+/* Routed experts on 8-bit rows q [T, H] with x_scale [T]: per pair (t, j) of top_k_index [T, k]
+ * (each in [0, E)) a = silu(gate) * up in fp32, in e4m3 with one power-of-two scale per 32
+ * columns (the least with amax <= 448 scale); y = bf16(a . down); out [T, H] =
+ * bf16(sum_j top_k_weights[t, j] y_tj). gate_up [E, 2I, H] and down [E, H, I] are e4m3 with row
+ * scales gu_scale [E, 2I] and dn_scale [E, H]; H and I multiples of 32, E <= 1024, k <= 64. */
+size_t moe_experts_fp8_workspace_bytes(int T, int H, int E, int k, int I);
+int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, int E, int k, int I,
+                            const long long* top_k_index, const void* top_k_weights,
+                            const void* gate_up, const float* gu_scale, const void* down,
+                            const float* dn_scale, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,7 @@ WEIGHTS_BF16 = 0
 WEIGHTS_FP8_E4M3 = 1
 ROUND_PRODUCT = 1
 EXACT_PRODUCT = 2
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # MOE_ACT_*
 NOALLOC_SCRATCH_BYTES = 16 << 20  # MOE_NOALLOC_SCRATCH_BYTES: moe_block_forward_noalloc's limit
 
 _P = ctypes.c_void_p
@@ -76,6 +77,13 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _P, _P, _F, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I,
          _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     ),
+    "moe_quantize_rows": (_I, [_P, _I, _I, _P, _P, _P]),
+    "moe_add_rmsnorm_fp8": (_I, [_P, _P, _P, _I, _I, _F, _P, _P, _P, _P, _P]),
+    "moe_linear": (
+        _I, [_P, _LL, _P, _P, _LL, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P, _P]),
+    "moe_experts_fp8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "moe_experts_fp8_forward": (
+        _I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 

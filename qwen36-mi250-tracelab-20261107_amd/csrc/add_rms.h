@@ -30,12 +30,11 @@ __device__ __forceinline__ void load_row(const uint16_t* src, int H, int lane, u
   }
 }
 
-// In place: tot (the x row) becomes total = bf16(x + h) when h is given (hv: the h row),
-// and y the normalised row, with w (wv) the norm weight row.
+// In place: tot (the x row) becomes total = bf16(x + h) when h is given (hv: the h row).
+// Returns rsqrt(mean(total^2) + eps).
 template <int HC>
-__device__ __forceinline__ void add_rms_compute(bool has_h, int H, float eps, uint4 (&tot)[HC],
-                                                const uint4 (&hv)[HC], const uint4 (&wv)[HC],
-                                                uint4 (&y)[HC]) {
+__device__ __forceinline__ float add_rms_sum(bool has_h, int H, float eps, uint4 (&tot)[HC],
+                                             const uint4 (&hv)[HC]) {
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < HC; ++c) {
@@ -51,7 +50,15 @@ __device__ __forceinline__ void add_rms_compute(bool has_h, int H, float eps, ui
     }
   }
   ss = wave_sum(ss);
-  const float r = rsqrtf(ss / (float)H + eps);
+  return rsqrtf(ss / (float)H + eps);
+}
+
+// add_rms_sum, and in y the normalised row, with w (wv) the norm weight row.
+template <int HC>
+__device__ __forceinline__ void add_rms_compute(bool has_h, int H, float eps, uint4 (&tot)[HC],
+                                                const uint4 (&hv)[HC], const uint4 (&wv)[HC],
+                                                uint4 (&y)[HC]) {
+  const float r = add_rms_sum<HC>(has_h, H, eps, tot, hv);
 #pragma unroll
   for (int c = 0; c < HC; ++c) {
     const uint32_t* t = &tot[c].x;

@@ -1,7 +1,7 @@
 // extern "C" entry points of libmoe_mi355x.so (declared in include/moe_mi355x.h).
 // Validation, workspace carving and the launch sequence of the MoE block; the kernels
-// live in route_sort.hip, expert_gemm.hip, prefill_gemm.hip, decode.hip, add_rms.hip and
-// combine.hip.
+// live in route_sort.hip, expert_gemm.hip, prefill_gemm.hip, decode.hip, add_rms.hip,
+// combine.hip, fp8_rows.hip and rows_gemm.hip.
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -15,6 +15,8 @@
 #include "add_rms.h"
 #include "expert_gemm.h"
 #include "decode.h"
+#include "fp8_rows.h"
+#include "rows_gemm.h"
 
 namespace moe {
 hipError_t launch_route(const uint16_t* logits, long long ld, int T, int E, int k, long long* idx64,
@@ -944,6 +946,52 @@ bool overlaps(const void* a, const void* b, size_t bytes) {
 }
 
 // The aliasing and alignment rules of the add + RMSNorm entry points.
+// The bytes an argument covers (p null: none), and whether outputs keep clear of the inputs and of
+// each other.
+struct Span {
+  const void* p;
+  long long bytes;
+};
+bool meets(const Span& a, const Span& b) {
+  if (!a.p || !b.p) return false;
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+bool apart(const Span* in, int ni, const Span* out, int no) {
+  for (int i = 0; i < no; ++i) {
+    for (int j = 0; j < ni; ++j)
+      if (meets(in[j], out[i])) return false;
+    for (int j = i + 1; j < no; ++j)
+      if (meets(out[i], out[j])) return false;
+  }
+  return true;
+}
+
+struct Experts8Ws {
+  int *counts, *offsets, *order, *table, *scratch;
+  uint8_t *aq, *asc;
+  uint16_t* y;
+  size_t bytes;
+  int MT, bm;
+};
+Experts8Ws carve_experts8(void* base, int T, int H, int E, int k, int I) {
+  Carver c{static_cast<char*>(base)};
+  Experts8Ws w{};
+  const int P = T * k;
+  w.bm = rows_tile_rows(T, k, E);
+  w.MT = max_tiles_of(T, k, E, w.bm, 0);
+  w.counts = c.take<int>(E);
+  w.offsets = c.take<int>(E);
+  w.order = c.take<int>(P);
+  w.table = c.take<int>(3 * (size_t)w.MT + 1);
+  w.scratch = c.take<int>(sort_scratch_bytes(P, E) / sizeof(int) + 1);
+  w.aq = c.take<uint8_t>((size_t)P * I);
+  w.asc = c.take<uint8_t>((size_t)((I + 127) / 128) * P * 4);
+  w.y = c.take<uint16_t>((size_t)P * H);
+  w.bytes = c.off;
+  return w;
+}
+
 int check_norm_args(const void* x, const void* h, const void* w, int T, int H, float eps,
                     const void* total, const void* norm, const void* out) {
   CHECK_ARG(T >= 0 && H > 0 && H % 8 == 0 && H <= 512 * kAddRmsMaxChunks,
@@ -1075,6 +1123,132 @@ int moe_block_forward_add_rms(const void* x, const void* h, const void* norm_wei
                        dn_scale, wdtype, sh_gate, sh_up, sh_down, nullptr, mode, out,
                        top_k_index, top_k_weights, logits, workspace, workspace_bytes, stream,
                        &nm);
+}
+
+int moe_quantize_rows(const void* x, int T, int n, void* q, float* scale, void* stream) {
+  CHECK_ARG(T >= 0 && n > 0 && n % 8 == 0 && n <= 512 * kAddRmsMaxChunks,
+            "quantize_rows: rows must be a positive multiple of 8 up to %d long (got %d)",
+            512 * kAddRmsMaxChunks, n);
+  if (T == 0) return MOE_OK;
+  CHECK_ARG(x && q && scale, "quantize_rows: null pointer");
+  CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)q % 8 == 0 && (uintptr_t)scale % 4 == 0,
+            "quantize_rows: x must be 16-byte aligned, q 8-byte and scale 4-byte");
+  const Span in{x, 2LL * T * n}, out[] = {{q, (long long)T * n}, {scale, 4LL * T}};
+  CHECK_ARG(apart(&in, 1, out, 2), "quantize_rows: outputs must not overlap the input or each other");
+  return hip_check(launch_quantize_rows(static_cast<const uint16_t*>(x), T, n,
+                                        static_cast<uint8_t*>(q), scale, (hipStream_t)stream),
+                   "quantize_rows launch");
+}
+
+int moe_add_rmsnorm_fp8(const void* x, const void* h, const void* weight, int T, int H, float eps,
+                        void* total, void* q, float* scale, void* norm, void* stream) {
+  CHECK_ARG(T >= 0 && H > 0 && H % 8 == 0 && H <= 512 * kAddRmsMaxChunks,
+            "add_rms_fp8: H must be a positive multiple of 8 up to %d (got %d)",
+            512 * kAddRmsMaxChunks, H);
+  CHECK_ARG(eps >= 0.f, "add_rms_fp8: eps must be >= 0 (got %g)", (double)eps);
+  if (T == 0) return MOE_OK;
+  CHECK_ARG(x && weight && q && scale && (!h || total), "add_rms_fp8: null pointer");
+  if (!h) total = nullptr;
+  CHECK_ARG(((uintptr_t)x | (uintptr_t)h | (uintptr_t)weight | (uintptr_t)total | (uintptr_t)norm) %
+                        16 == 0 && (uintptr_t)q % 8 == 0 && (uintptr_t)scale % 4 == 0,
+            "add_rms_fp8: bf16 rows must be 16-byte aligned, q 8-byte and scale 4-byte");
+  const long long n = (long long)T * H;
+  const Span in[] = {{x, 2 * n}, {h, 2 * n}, {weight, 2LL * H}};
+  const Span out[] = {{total, 2 * n}, {q, n}, {scale, 4LL * T}, {norm, 2 * n}};
+  CHECK_ARG(apart(in, 3, out, 4), "add_rms_fp8: outputs must not overlap the inputs or each other");
+  return hip_check(launch_add_rms_fp8(static_cast<const uint16_t*>(x),
+                                      static_cast<const uint16_t*>(h),
+                                      static_cast<const uint16_t*>(weight), T, H, eps,
+                                      static_cast<uint16_t*>(total), static_cast<uint8_t*>(q),
+                                      scale, static_cast<uint16_t*>(norm), (hipStream_t)stream),
+                   "add_rms_fp8 launch");
+}
+
+int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
+               const float* w_scale, int dtype, int M, int K, int N, const void* bias,
+               int bias_f32, int act, const void* mul, const void* residual, void* out,
+               void* stream) {
+  CHECK_ARG(dtype == MOE_WEIGHTS_BF16 || dtype == MOE_WEIGHTS_FP8_E4M3, "linear: bad dtype %d",
+            dtype);
+  const int es = dtype == MOE_WEIGHTS_BF16 ? 2 : 1;
+  CHECK_ARG(M >= 0 && N >= 0, "linear: M and N must be >= 0 (got %d, %d)", M, N);
+  CHECK_ARG(K >= 16 / es && K % (16 / es) == 0 && K <= (1 << 28),
+            "linear: K must be a positive multiple of %d (got %d)", 16 / es, K);
+  CHECK_ARG(act >= MOE_ACT_NONE && act <= MOE_ACT_GELU_TANH, "linear: bad activation %d", act);
+  if (M == 0 || N == 0) return MOE_OK;
+  CHECK_ARG(x && w && out, "linear: null pointer");
+  CHECK_ARG((es == 1) == (x_scale != nullptr) && (es == 1) == (w_scale != nullptr),
+            "linear: e4m3 operands take x_scale and w_scale, bf16 ones neither");
+  CHECK_ARG(ldx >= K && ldw >= K && ldx * es % 16 == 0 && ldw * es % 16 == 0 &&
+                ((uintptr_t)x | (uintptr_t)w) % 16 == 0,
+            "linear: rows of x and w must start at multiples of 16 bytes, ldx and ldw >= K");
+  CHECK_ARG((((uintptr_t)out | (uintptr_t)mul | (uintptr_t)residual) % 8) == 0 &&
+                (uintptr_t)bias % (bias_f32 ? 4 : 2) == 0,
+            "linear: out, mul and residual must be 8-byte aligned");
+  const long long n = 2LL * M * N;
+  const Span in[] = {{x, ((M - 1) * ldx + K) * es}, {w, ((N - 1) * ldw + K) * es},
+                     {x_scale, 4LL * M}, {w_scale, 4LL * N}, {bias, (bias_f32 ? 4LL : 2LL) * N},
+                     {mul, n}, {residual, n}};
+  const Span o{out, n};
+  CHECK_ARG(apart(in, 7, &o, 1), "linear: out must not overlap the inputs");
+  RowsGemm a{};
+  a.x = static_cast<const uint8_t*>(x), a.ldx = ldx * es;
+  a.w = static_cast<const uint8_t*>(w), a.ldw = ldw * es;
+  a.xs = x_scale, a.ws = w_scale;
+  a.M = M, a.N = N, a.Kb = K * es;
+  a.bias = bias, a.bias_f32 = bias_f32, a.act = act;
+  a.mul = static_cast<const uint16_t*>(mul), a.res = static_cast<const uint16_t*>(residual);
+  a.out = static_cast<uint16_t*>(out);
+  const hipError_t err = launch_rows_gemm(kRowsLinear, es, a, 0, (hipStream_t)stream);
+  if (err == hipErrorInvalidValue)
+    return fail(MOE_EINVAL, "linear: no kernel configuration for M=%d K=%d N=%d", M, K, N);
+  return hip_check(err, "linear launch");
+}
+
+size_t moe_experts_fp8_workspace_bytes(int T, int H, int E, int k, int I) {
+  if (T < 0 || k < 1 || E < 1 || H < 1 || I < 1 || (long long)T * k >= (1LL << 30)) return 0;
+  return carve_experts8(nullptr, T, H, E, k, I).bytes;
+}
+
+int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, int E, int k, int I,
+                            const long long* top_k_index, const void* top_k_weights,
+                            const void* gate_up, const float* gu_scale, const void* down,
+                            const float* dn_scale, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  int rc = check_experts_shape(T, H, E, k, I);
+  if (rc) return rc;
+  if (T == 0) return MOE_OK;
+  CHECK_ARG(q && x_scale && top_k_index && top_k_weights && gate_up && gu_scale && down &&
+                dn_scale && out,
+            "experts_fp8: null pointer");
+  CHECK_ARG(((uintptr_t)q | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)out |
+             (uintptr_t)workspace) % 16 == 0,
+            "experts_fp8: q, the weights, out and the workspace must be 16-byte aligned");
+  const Experts8Ws w = carve_experts8(workspace, T, H, E, k, I);
+  CHECK_ARG(workspace && workspace_bytes >= w.bytes, "experts_fp8: workspace too small: %zu < %zu",
+            workspace_bytes, w.bytes);
+  hipStream_t s = (hipStream_t)stream;
+  HIP_TRY(launch_route_sort(nullptr, 0, nullptr, top_k_index, T, E, k, w.bm, 0, nullptr, nullptr,
+                            nullptr, w.counts, w.offsets, w.order, w.table, w.MT, w.scratch, s),
+          "sort launch");
+  RowsGemm a{};
+  a.x = static_cast<const uint8_t*>(q), a.ldx = H;
+  a.w = static_cast<const uint8_t*>(gate_up), a.ldw = H, a.estride = 2LL * I * H;
+  a.xs = x_scale, a.ws = gu_scale;
+  a.N = I, a.Kb = H;
+  a.table = w.table, a.order = w.order, a.MT = w.MT, a.topk = k;
+  a.P = (long long)T * k;
+  a.aq = w.aq, a.asc = w.asc;
+  HIP_TRY(launch_rows_gemm(kRowsGateUp, 1, a, w.bm, s), "gate_up launch");
+  a.x = w.aq, a.ldx = I;
+  a.w = static_cast<const uint8_t*>(down), a.ldw = I, a.estride = (long long)H * I;
+  a.xs = nullptr, a.ws = dn_scale;
+  a.N = H, a.Kb = I;
+  a.out = w.y;
+  HIP_TRY(launch_rows_gemm(kRowsDown, 1, a, w.bm, s), "down launch");
+  return hip_check(launch_combine(w.y, static_cast<const uint16_t*>(top_k_weights), k, nullptr,
+                                  nullptr, 0, nullptr, static_cast<uint16_t*>(out), T, H, 0, s),
+                   "combine launch");
 }
 
 }  // extern "C"

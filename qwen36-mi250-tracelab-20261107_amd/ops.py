@@ -17,6 +17,13 @@ caching allocator; weights are read in place. Nothing here synchronises with the
   decode_gate_up     top-k + routed gate_up, T <= 4      (engine/fast/fused.py:554-632)
   decode_down        down + combine + shared, T <= 4     (engine/fast/fused.py:635-692)
   add_rms            residual add + RMSNorm              (engine/fast/kernels.py:636-650)
+
+8-bit activations (no counterpart in the reference, whose activations are bf16):
+
+  quantize_rows      bf16 rows -> e4m3 rows with fp32 scales
+  add_rms_fp8        add_rms with the norm as e4m3 rows
+  linear             residual + mul * act(x @ w.T + bias), bf16 or e4m3 operands
+  experts_fp8        routed experts on e4m3 rows
 """
 
 from __future__ import annotations
@@ -408,3 +415,171 @@ def add_rms(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, eps: 
                                       ptr(total) if h2 is not None else None, ptr(out),
                                       stream_of(x2)), "add_rms")
     return total.reshape(x.shape), out.reshape(x.shape)
+
+
+# ------------------------------------------------------------------------- 8-bit activations
+
+
+def _same_device(first: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the input on {first.device}")
+
+
+def _call(name: str, device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``device`` current: a launch goes to the current device."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous, at a multiple of 16 bytes (a view into a larger tensor may not be)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _scales(t, name: str, n: int) -> torch.Tensor:
+    if t is None or t.dtype != torch.float32 or t.numel() != n:
+        raise ValueError(f"{name} must be {n} float32 values")
+    return t.contiguous()
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q float8_e4m3fn [..., n], scale fp32 [...]) of ``x`` [..., n] bf16: per row
+    scale = amax / 448 over the finite values (1 for a row of zeros; amax counts as 2^-100 at
+    least) and q = e4m3(x / scale), ties to even. NaN and infinite values become NaN. The format
+    of ``fp8.quantize_rows``, for activations."""
+    _need_cuda(x)
+    x2 = _aligned(_bf16(x, "x").reshape(-1, x.shape[-1]))
+    rows, n = x2.shape
+    q = torch.empty(x.shape, dtype=FP8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call("quantize_rows", x.device, _lib.load().moe_quantize_rows, x2.data_ptr(), rows, n,
+          q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def add_rms_fp8(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
+                return_norm: bool = False):
+    """``add_rms`` with the norm in 8 bits: (total, q, scale), and with ``return_norm`` the
+    bf16 norm as a fourth item (what a bf16 router reads). q and scale are ``quantize_rows`` of
+    the fp32 norm: it is rounded once, not to bf16 first."""
+    _need_cuda(x, h, weight)
+    _same_device(x, h=h, weight=weight)
+    x2 = _aligned(_bf16(x, "x").reshape(-1, x.shape[-1]))
+    rows, n = x2.shape
+    if h is not None and h.shape != x.shape:
+        raise ValueError(f"h has shape {tuple(h.shape)}, x {tuple(x.shape)}")
+    h2 = None if h is None else _aligned(_bf16(h, "h"))
+    w = _aligned(_bf16(weight, "weight"))
+    if w.numel() != n:
+        raise ValueError(f"weight must have {n} elements (got {w.numel()})")
+    total = x2 if h2 is None else torch.empty_like(x2)
+    q = torch.empty(x.shape, dtype=FP8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    norm = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if return_norm else None
+    _call("add_rms_fp8", x.device, _lib.load().moe_add_rmsnorm_fp8, x2.data_ptr(), ptr(h2),
+          w.data_ptr(), rows, n, float(eps), None if h2 is None else total.data_ptr(),
+          q.data_ptr(), scale.data_ptr(), ptr(norm))
+    total = total.view(x.shape)
+    return (total, q, scale, norm) if return_norm else (total, q, scale)
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = None,
+           w_scale: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+           activation: str | None = None, mul: torch.Tensor | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``bf16(residual + mul * act(x @ w.T + bias))`` [..., N] for ``x`` [..., K] and ``w``
+    [N, K], fp32 up to the one rounding. Operands are both bf16 (K a multiple of 8) or both
+    float8_e4m3fn with fp32 row scales ``x_scale`` [...] and ``w_scale`` [N] (K a multiple of
+    16). ``bias`` [N] is bf16 or fp32, ``mul`` and ``residual`` [..., N] bf16; ``activation`` is
+    None, "relu", "silu", "gelu" or "gelu_tanh". Rows of ``w`` (and of a 2-D ``x``) may be
+    strided, as in a slice of a packed weight, if each starts at a multiple of 16 bytes."""
+    _need_cuda(x, w)
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(_lib.ACTIVATIONS)} (got {activation!r})")
+    if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, FP8):
+        raise ValueError(f"x and w must both be bfloat16 or float8_e4m3fn (got {x.dtype}, {w.dtype})")
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not match")
+    _same_device(x, w=w, x_scale=x_scale, w_scale=w_scale, bias=bias, mul=mul, residual=residual)
+    n, k = w.shape
+    size = x.element_size()
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    rows = x2.shape[0]
+    if x2.stride(1) != 1 or x2.stride(0) < k or x2.stride(0) * size % 16 or x2.data_ptr() % 16:
+        x2 = _aligned(x2)
+    if w.stride(1) != 1 or w.stride(0) < k or w.stride(0) * size % 16 or w.data_ptr() % 16:
+        raise ValueError("rows of w must be contiguous and start at multiples of 16 bytes")
+    dtype = _lib.WEIGHTS_BF16
+    if x.dtype == FP8:
+        dtype = _lib.WEIGHTS_FP8_E4M3
+        x_scale, w_scale = _scales(x_scale, "x_scale", rows), _scales(w_scale, "w_scale", n)
+    elif x_scale is not None or w_scale is not None:
+        raise ValueError("bf16 operands take no scales")
+    if bias is not None:
+        if bias.dtype not in (torch.bfloat16, torch.float32) or bias.numel() != n:
+            raise ValueError(f"bias must be {n} bfloat16 or float32 values")
+        bias = bias.contiguous()
+    shape = (*x.shape[:-1], n)
+    for name, t in (("mul", mul), ("residual", residual)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, the output {shape}")
+    if mul is not None:
+        mul = _aligned(_bf16(mul, "mul"))
+    if residual is not None:
+        residual = _aligned(_bf16(residual, "residual"))
+    out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    _call("linear", x.device, _lib.load().moe_linear, x2.data_ptr(), x2.stride(0), ptr(x_scale),
+          w.data_ptr(), w.stride(0), ptr(w_scale), dtype, rows, k, n, ptr(bias),
+          int(bias is not None and bias.dtype == torch.float32), _lib.ACTIVATIONS[activation],
+          ptr(mul), ptr(residual), out.data_ptr())
+    return out
+
+
+def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
+                top_k_weights: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, *,
+                gate_up_scale: torch.Tensor, down_scale: torch.Tensor) -> torch.Tensor:
+    """Routed-expert output [T, H] bf16 for e4m3 rows ``q`` [T, H] with ``scale`` [T]
+    (``add_rms_fp8``, ``quantize_rows``) and e4m3 experts (``fp8.quantize_experts``): both
+    products on the e4m3 matrix instructions. Between them a = silu(gate) * up, fp32, goes in e4m3
+    with one power-of-two scale per 32 columns; pair outputs are rounded to bf16 and their weighted
+    sum, fp32 with bf16 weights, once more. ``top_k_index`` [T, k] int64 holds experts in
+    [0, E)."""
+    _need_cuda(q, scale, top_k_index, top_k_weights, gate_up, down)
+    _same_device(q, scale=scale, top_k_index=top_k_index, top_k_weights=top_k_weights,
+                 gate_up=gate_up, down=down, gate_up_scale=gate_up_scale, down_scale=down_scale)
+    if q.dtype != FP8 or q.dim() != 2:
+        raise ValueError(f"q must be float8_e4m3fn [T, H] (got {q.dtype}, {tuple(q.shape)})")
+    if gate_up.dtype != FP8 or down.dtype != FP8:
+        raise ValueError("experts_fp8 takes float8_e4m3fn experts (see fp8.quantize_experts)")
+    gu, gus, _ = expert_weight(gate_up, gate_up_scale, "gate_up")
+    dn, dns, _ = expert_weight(down, down_scale, "down")
+    _check_row_major(gu, dn)
+    tokens, hidden = q.shape
+    if gu.dim() != 3 or gu.shape[2] != hidden or gu.shape[1] % 2:
+        raise ValueError(f"gate_up shape {tuple(gu.shape)} does not fit rows of {hidden}")
+    nexp, inter = gu.shape[0], gu.shape[1] // 2
+    if dn.shape != (nexp, hidden, inter):
+        raise ValueError(f"down shape {tuple(dn.shape)} != {(nexp, hidden, inter)}")
+    if top_k_index.dtype != torch.long or top_k_index.dim() != 2 or top_k_index.shape[0] != tokens:
+        raise ValueError(f"top_k_index must be int64 [{tokens}, k]")
+    if top_k_weights.shape != top_k_index.shape:
+        raise ValueError(f"top_k_weights must be {tuple(top_k_index.shape)}")
+    top_k = top_k_index.shape[1]
+    scale = _scales(scale, "scale", tokens)
+    q = _aligned(q)
+    idx = top_k_index.contiguous()
+    wts = top_k_weights.to(torch.bfloat16).contiguous()
+    out = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=q.device)
+    lib = _lib.load()
+    nbytes = lib.moe_experts_fp8_workspace_bytes(tokens, hidden, nexp, top_k, inter)
+    # a workspace of the call's own: one captured in a graph belongs to that graph
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+    _call("experts_fp8", q.device, lib.moe_experts_fp8_forward, q.data_ptr(), scale.data_ptr(), tokens,
+          hidden, nexp, top_k, inter, idx.data_ptr(), wts.data_ptr(), gu.data_ptr(), gus.data_ptr(),
+          dn.data_ptr(), dns.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
+    return out
