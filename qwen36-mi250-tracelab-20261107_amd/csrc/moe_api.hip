@@ -1182,9 +1182,9 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
   CHECK_ARG(ldx >= K && ldw >= K && ldx * es % 16 == 0 && ldw * es % 16 == 0 &&
                 ((uintptr_t)x | (uintptr_t)w) % 16 == 0,
             "linear: rows of x and w must start at multiples of 16 bytes, ldx and ldw >= K");
-  CHECK_ARG((((uintptr_t)out | (uintptr_t)mul | (uintptr_t)residual) % 8) == 0 &&
+  CHECK_ARG((((uintptr_t)out | (uintptr_t)mul | (uintptr_t)residual) % 16) == 0 &&
                 (uintptr_t)bias % (bias_f32 ? 4 : 2) == 0,
-            "linear: out, mul and residual must be 8-byte aligned");
+            "linear: out, mul and residual must be 16-byte aligned, bias as its type");
   const long long n = 2LL * M * N;
   const Span in[] = {{x, ((M - 1) * ldx + K) * es}, {w, ((N - 1) * ldw + K) * es},
                      {x_scale, 4LL * M}, {w_scale, 4LL * N}, {bias, (bias_f32 ? 4LL : 2LL) * N},
@@ -1232,7 +1232,7 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
                             nullptr, w.counts, w.offsets, w.order, w.table, w.MT, w.scratch, s),
           "sort launch");
   RowsGemm a{};
-  a.x = static_cast<const uint8_t*>(q), a.ldx = H;
+  a.x = static_cast<const uint8_t*>(q), a.ldx = H, a.xbytes = (long long)T * H;
   a.w = static_cast<const uint8_t*>(gate_up), a.ldw = H, a.estride = 2LL * I * H;
   a.xs = x_scale, a.ws = gu_scale;
   a.N = I, a.Kb = H;

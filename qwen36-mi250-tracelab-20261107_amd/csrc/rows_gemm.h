@@ -39,6 +39,7 @@ struct RowsGemm {
   long long ldw, estride;
   const float* xs;    // a scale per token row, per weight row (e4m3 only)
   const float* ws;
+  long long xbytes;   // of all token rows (kRowsGateUp)
   int M, N;           // token rows (kRowsLinear); outputs of a token (kRowsGateUp: I)
   int Kb;             // bytes of a row, a multiple of 16
   // kRowsLinear
@@ -78,97 +79,162 @@ __device__ __forceinline__ f32x4_t rows_mma_scaled(uint4 a0, uint4 a1, uint4 b0,
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f, 0, sb);
 }
 
-// v sigmoid(t) with exp of a negative argument only: tiny results stay where exp(-t) would
-// overflow.
+// v sigmoid(t), as v / (1 + e) or v e / (1 + e) with e = exp(-|t|) <= 1, from the hardware's exp2 and
+// reciprocal. e is squared from exp2(-|t| log2(e) / 2), with that argument's rounding error put back:
+// so v e may be tiny where e alone would be lost (the hardware's exp2 has no subnormal results).
 __device__ __forceinline__ float rows_gate(float v, float t) {
-  const float e = expf(-fabsf(t));
-  return v * ((t < 0.f ? e : 1.0f) / (1.0f + e));
+  constexpr float kHalfL2e = -0.721347520444481703680f;
+  const float x = fminf(fabsf(t), 256.f);
+  const float p = x * kHalfL2e;
+  const float h = __builtin_amdgcn_exp2f(p) *
+                  fmaf(fmaf(x, kHalfL2e, -p), 0.693147182464599609375f, 1.0f);
+  const float f = t < 0.f ? h : 1.0f;
+  return v * f * f * __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
 }
-// gelu_tanh as v sigmoid(2 u), u = sqrt(2 / pi) (v + 0.044715 v^3), and gelu by erfc: the sums
-// 1 + tanh and 1 + erf lose the digits of a negative v's small results.
+// The activations, by the code that they share: relu and none; silu and gelu_tanh, v sigmoid(t) with
+// t = v or 2 sqrt(2 / pi) (v + 0.044715 v^3); gelu by erfc. (The sums 1 + tanh and 1 + erf would lose
+// the digits of a negative v's small results.)
+enum RowsActClass { kClassLinear, kClassGate, kClassErf };
+__host__ __device__ inline RowsActClass rows_act_class(int act) {
+  return act == kActGelu ? kClassErf : act >= kActSilu ? kClassGate : kClassLinear;
+}
+template <int CLASS>
 __device__ __forceinline__ float rows_act(float v, int act) {
-  switch (act) {
-    case kActRelu:
-      return v < 0.f ? 0.f : v;  // NaN stays NaN
-    case kActSilu:
-      return rows_gate(v, v);
-    case kActGelu:
-      return 0.5f * v * erfcf(v * -0.70710678118654752f);
-    case kActGeluTanh:
-      return rows_gate(v, 1.5957691216057308f * fmaf(0.044715f * v * v, v, v));
+  if (CLASS == kClassErf) return 0.5f * v * erfcf(v * -0.70710678118654752f);
+  if (CLASS == kClassGate) {
+    const float c0 = act == kActSilu ? 1.0f : 1.5957691216057308f;
+    const float c1 = act == kActSilu ? 0.0f : 1.5957691216057308f * 0.044715f;
+    return rows_gate(v, v * fmaf(c1, v * v, c0));
   }
-  return v;
+  return act == kActRelu && v < 0.f ? 0.f : v;  // NaN stays NaN
 }
 
-// kRowsLinear: outputs n .. n + 3 (as far as N goes) of token row m.
-__device__ __forceinline__ void rows_linear_out(const RowsGemm& a, long long m, int n, f32x4_t acc) {
+// kRowsLinear: C neighbouring outputs of token row m from n on (as far as N goes), whose sums are v.
+// VEC: N is a multiple of C, so a row's C outputs are one aligned access.
+template <int CLASS, int C, bool VEC>
+__device__ __forceinline__ void rows_linear_out(const RowsGemm& a, long long m, int n, float xs,
+                                                const float (&ws)[C], const float (&bias)[C],
+                                                float (&v)[C]) {
+  static_assert(C == 4 || C == 8, "8 or 16 bytes");
   if (n >= a.N) return;
-  const float xs = a.xs ? a.xs[m] : 1.f;
   const long long at = m * a.N + n;
-  const bool whole = a.N % 4 == 0;  // then 8-byte accesses are aligned and n + 3 < N
-  uint2 mv = make_uint2(0u, 0u), rv = make_uint2(0u, 0u);
-  if (whole) {
-    if (a.mul) mv = *reinterpret_cast<const uint2*>(a.mul + at);
-    if (a.res) rv = *reinterpret_cast<const uint2*>(a.res + at);
+  uint16_t mv[C], rv[C];
+  auto load = [&](const uint16_t* p, uint16_t (&d)[C]) __attribute__((always_inline)) {
+    if (VEC) {
+      if (C == 8)
+        __builtin_memcpy(d, __builtin_assume_aligned(p + at, 16), 16);
+      else
+        __builtin_memcpy(d, __builtin_assume_aligned(p + at, 8), 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] = n + i < a.N ? p[at + i] : 0;
+    }
+  };
+  if (a.mul) load(a.mul, mv);
+  if (a.res) load(a.res, rv);
+  if (a.ws) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] *= xs * ws[i];
   }
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += bias[i];
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = rows_act<CLASS>(v[i], a.act);
+  if (a.mul) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] *= bf_bits2f(mv[i]);
+  }
+  if (a.res) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += bf_bits2f(rv[i]);
+  }
+  uint32_t o[C / 2];
+#pragma unroll
+  for (int i = 0; i < C; i += 2) o[i / 2] = pack_bf2_rne(v[i], v[i + 1]);
+  if (VEC) {
+    if (C == 8)
+      st16(a.out + at, make_uint4(o[0], o[1], o[C / 2 - 2], o[C / 2 - 1]));
+    else
+      *reinterpret_cast<uint2*>(a.out + at) = make_uint2(o[0], o[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < a.N) a.out[at + i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
+  }
+}
+// Their weight scales and biases (zeros past N).
+template <int C>
+__device__ __forceinline__ void rows_linear_cols(const RowsGemm& a, int n, float (&ws)[C],
+                                                 float (&bias)[C]) {
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const bool in = n + i < a.N;
+    ws[i] = a.ws && in ? a.ws[n + i] : 0.f;
+    bias[i] = !a.bias || !in ? 0.f
+              : a.bias_f32   ? static_cast<const float*>(a.bias)[n + i]
+                             : bf_bits2f(static_cast<const uint16_t*>(a.bias)[n + i]);
+  }
+}
+
+// The group format's scale 2^z of a group with that amax: the least with amax <= 448 2^z, so that no
+// value saturates.
+__device__ __forceinline__ int group_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  return max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
+}
+// v / 2^z in e4m3; non-finite values become NaN (v * 0 is NaN).
+__device__ __forceinline__ uint32_t pack_group4(const float (&v)[4], float m) {
   float o[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = n + i < a.N;
-    float v = acc[i];
-    if (a.ws) v *= xs * (in ? a.ws[n + i] : 0.f);
-    if (a.bias && in)
-      v += a.bias_f32 ? static_cast<const float*>(a.bias)[n + i]
-                      : bf_bits2f(static_cast<const uint16_t*>(a.bias)[n + i]);
-    v = rows_act(v, a.act);
-    const uint32_t mw = i < 2 ? mv.x : mv.y, rw = i < 2 ? rv.x : rv.y;
-    if (a.mul) v *= whole ? (i & 1 ? bf_hi(mw) : bf_lo(mw)) : in ? bf_bits2f(a.mul[at + i]) : 0.f;
-    if (a.res) v += whole ? (i & 1 ? bf_hi(rw) : bf_lo(rw)) : in ? bf_bits2f(a.res[at + i]) : 0.f;
-    o[i] = v;
-  }
-  const uint2 p = make_uint2(pack_bf2_rne(o[0], o[1]), pack_bf2_rne(o[2], o[3]));
-  if (whole) {
-    *reinterpret_cast<uint2*>(a.out + at) = p;
-  } else {
-    const uint32_t u[2] = {p.x, p.y};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) a.out[at + i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
-  }
+  for (int i = 0; i < 4; ++i) o[i] = fmaf(v[i], 0.f, v[i] * m);
+  return pack_e4m3(o[0], o[1], o[2], o[3]);
 }
 
-// kRowsGateUp: group grp (32 columns) of sorted row r, whose values the four lanes of one lr
-// hold: g[h], u[h] columns 16 h + 4 kq .. + 3. Every lane of the wave calls; live: the row is
-// stored. The scale 2^z is the least power of two with amax <= 448 2^z, so no value saturates;
-// a non-finite value becomes NaN (v * 0 is NaN) and does not count for the amax.
+// kRowsGateUp: C quads of four columns each of sorted row r from column n on, of which a group's
+// columns lie in LANES lanes 16 apart (1 << s of them): the quads of one lane are stride columns
+// apart. Every lane of the wave calls; live: the row is stored. Scales of the groups that fill
+// up the last 128 columns are written as 1 (their values are read as zeros).
+template <int C, int LANES, int STRIDE>
 __device__ __forceinline__ void rows_gate_up_out(const RowsGemm& a, bool live, long long r, int e,
-                                                 float xs, int grp, int kq, const f32x4_t (&g)[2],
-                                                 const f32x4_t (&u)[2]) {
-  const float* sg = a.ws + (long long)e * 2 * a.N + grp * 32 + 4 * kq;
+                                                 float xs, int n, const f32x4_t (&g)[C],
+                                                 const f32x4_t (&u)[C]) {
+  static_assert(C * 4 * LANES == 32, "one group");
+  const bool in = n < a.N;  // a multiple of 32: the whole group
+  const float* sg = a.ws + (long long)e * 2 * a.N + (in ? n : 0);
   const float* su = sg + a.N;
-  float v[2][4], amax = 0.f;
+  float v[C][4], amax = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < C; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float gv = g[h][i] * (xs * sg[16 * h + i]), uv = u[h][i] * (xs * su[16 * h + i]);
+      const float gv = g[h][i] * (xs * sg[STRIDE * h + i]);
+      const float uv = u[h][i] * (xs * su[STRIDE * h + i]);
       v[h][i] = rows_gate(gv, gv) * uv;
       amax = fmaxf(amax, finite_abs(v[h][i]));
     }
-  amax = fmaxf(amax, __shfl_xor(amax, 16));
-  amax = fmaxf(amax, __shfl_xor(amax, 32));
-  const uint32_t bits = __float_as_uint(amax);
-  const int z = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
+#pragma unroll
+  for (int x = 16; x < 16 * LANES; x *= 2) amax = fmaxf(amax, __shfl_xor(amax, x));
+  const int z = group_exponent(amax);
   const float m = __uint_as_float((uint32_t)(127 - z) << 23);
   if (!live) return;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[h][i] = fmaf(v[h][i], 0.f, v[h][i] * m);
-    *reinterpret_cast<uint32_t*>(a.aq + r * a.N + grp * 32 + 16 * h + 4 * kq) =
-        pack_e4m3(v[h][0], v[h][1], v[h][2], v[h][3]);
+  uint8_t* sc = a.asc + ((n >> 7) * a.P + r) * 4 + (n >> 5 & 3);
+  if (!in) {
+    *sc = 127;
+    return;
   }
-  if (kq == 0) a.asc[((grp >> 2) * a.P + r) * 4 + (grp & 3)] = (uint8_t)(z + 127);
+  uint32_t q[C];
+#pragma unroll
+  for (int h = 0; h < C; ++h) q[h] = pack_group4(v[h], m);
+  uint8_t* out = a.aq + r * a.N + n;
+  if (C == 4 && STRIDE == 4) {
+    st16(out, make_uint4(q[0], q[1], q[2], q[3]));
+  } else {
+#pragma unroll
+    for (int h = 0; h < C; ++h) *reinterpret_cast<uint32_t*>(out + STRIDE * h) = q[h];
+  }
+  *sc = (uint8_t)(z + 127);  // all lanes of a group the same
 }
 
 // kRowsDown: outputs n .. n + 3 of pair row p.
