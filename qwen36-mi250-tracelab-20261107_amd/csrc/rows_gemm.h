@@ -26,6 +26,7 @@
 
 #include "fp8_rows.h"
 #include "moe_common.h"
+#include "route_sort_dev.h"
 
 namespace moe {
 
@@ -94,54 +95,49 @@ __device__ __forceinline__ float rows_gate(float v, float t) {
 // The activations, by the code that they share: relu and none; silu and gelu_tanh, v sigmoid(t) with
 // t = v or 2 sqrt(2 / pi) (v + 0.044715 v^3); gelu by erfc. (The sums 1 + tanh and 1 + erf would lose
 // the digits of a negative v's small results.)
-enum RowsActClass { kClassLinear, kClassGate, kClassErf };
-__host__ __device__ inline RowsActClass rows_act_class(int act) {
-  return act == kActGelu ? kClassErf : act >= kActSilu ? kClassGate : kClassLinear;
-}
-template <int CLASS>
-__device__ __forceinline__ float rows_act(float v, int act) {
-  if (CLASS == kClassErf) return 0.5f * v * erfcf(v * -0.70710678118654752f);
-  if (CLASS == kClassGate) {
+template <int C>
+__device__ __forceinline__ void rows_act(float (&v)[C], int act) {
+  if (act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+  } else if (act >= kActSilu) {
     const float c0 = act == kActSilu ? 1.0f : 1.5957691216057308f;
     const float c1 = act == kActSilu ? 0.0f : 1.5957691216057308f * 0.044715f;
-    return rows_gate(v, v * fmaf(c1, v * v, c0));
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = rows_gate(v[i], v[i] * fmaf(c1, v[i] * v[i], c0));
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
   }
-  return act == kActRelu && v < 0.f ? 0.f : v;  // NaN stays NaN
 }
 
-// kRowsLinear: C neighbouring outputs of token row m from n on (as far as N goes), whose sums are v.
-// VEC: N is a multiple of C, so a row's C outputs are one aligned access.
-template <int CLASS, int C, bool VEC>
+// kRowsLinear: C neighbouring outputs of token row m from n on (as far as N goes), whose sums are
+// v. Where N is a multiple of C they are one aligned access.
+template <int C>
 __device__ __forceinline__ void rows_linear_out(const RowsGemm& a, long long m, int n, float xs,
                                                 const float (&ws)[C], const float (&bias)[C],
                                                 float (&v)[C]) {
   static_assert(C == 4 || C == 8, "8 or 16 bytes");
-  if (n >= a.N) return;
   const long long at = m * a.N + n;
-  uint16_t mv[C], rv[C];
+  const bool vec = a.N % C == 0;
   auto load = [&](const uint16_t* p, uint16_t (&d)[C]) __attribute__((always_inline)) {
-    if (VEC) {
-      if (C == 8)
-        __builtin_memcpy(d, __builtin_assume_aligned(p + at, 16), 16);
-      else
-        __builtin_memcpy(d, __builtin_assume_aligned(p + at, 8), 8);
+    if (vec) {
+      __builtin_memcpy(d, __builtin_assume_aligned(p + at, 2 * C), 2 * C);
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i) d[i] = n + i < a.N ? p[at + i] : 0;
     }
   };
+  uint16_t mv[C], rv[C];
   if (a.mul) load(a.mul, mv);
   if (a.res) load(a.res, rv);
   if (a.ws) {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] *= xs * ws[i];
   }
-  if (a.bias) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] += bias[i];
-  }
-#pragma unroll
-  for (int i = 0; i < C; ++i) v[i] = rows_act<CLASS>(v[i], a.act);
+  for (int i = 0; i < C; ++i) v[i] += bias[i];
+  rows_act(v, a.act);
   if (a.mul) {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] *= bf_bits2f(mv[i]);
@@ -153,11 +149,8 @@ __device__ __forceinline__ void rows_linear_out(const RowsGemm& a, long long m, 
   uint32_t o[C / 2];
 #pragma unroll
   for (int i = 0; i < C; i += 2) o[i / 2] = pack_bf2_rne(v[i], v[i + 1]);
-  if (VEC) {
-    if (C == 8)
-      st16(a.out + at, make_uint4(o[0], o[1], o[C / 2 - 2], o[C / 2 - 1]));
-    else
-      *reinterpret_cast<uint2*>(a.out + at) = make_uint2(o[0], o[1]);
+  if (vec) {
+    __builtin_memcpy(__builtin_assume_aligned(a.out + at, 2 * C), o, 2 * C);
   } else {
 #pragma unroll
     for (int i = 0; i < C; ++i)
@@ -184,66 +177,51 @@ __device__ __forceinline__ int group_exponent(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   return max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
 }
-// v / 2^z in e4m3; non-finite values become NaN (v * 0 is NaN).
-__device__ __forceinline__ uint32_t pack_group4(const float (&v)[4], float m) {
-  float o[4];
+// kRowsGateUp: columns n .. n + 7 of sorted row r, whose sums are g and u and whose scales sg and su
+// (the token's included); the four lanes of a group of 32 are neighbours. Every lane of the wave
+// calls; live: the row is stored. Scales of the groups that fill up the last 128 columns are
+// written as 1 (their values are read as zeros).
+__device__ __forceinline__ void rows_gate_up_out(const RowsGemm& a, bool live, long long r, int n,
+                                                 const float (&sg)[8], const float (&su)[8], float xs,
+                                                 const float (&g)[8], const float (&u)[8]) {
+  float v[8], amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = fmaf(v[i], 0.f, v[i] * m);
-  return pack_e4m3(o[0], o[1], o[2], o[3]);
-}
-
-// kRowsGateUp: C quads of four columns each of sorted row r from column n on, of which a group's
-// columns lie in LANES lanes 16 apart (1 << s of them): the quads of one lane are stride columns
-// apart. Every lane of the wave calls; live: the row is stored. Scales of the groups that fill
-// up the last 128 columns are written as 1 (their values are read as zeros).
-template <int C, int LANES, int STRIDE>
-__device__ __forceinline__ void rows_gate_up_out(const RowsGemm& a, bool live, long long r, int e,
-                                                 float xs, int n, const f32x4_t (&g)[C],
-                                                 const f32x4_t (&u)[C]) {
-  static_assert(C * 4 * LANES == 32, "one group");
-  const bool in = n < a.N;  // a multiple of 32: the whole group
-  const float* sg = a.ws + (long long)e * 2 * a.N + (in ? n : 0);
-  const float* su = sg + a.N;
-  float v[C][4], amax = 0.f;
-#pragma unroll
-  for (int h = 0; h < C; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float gv = g[h][i] * (xs * sg[STRIDE * h + i]);
-      const float uv = u[h][i] * (xs * su[STRIDE * h + i]);
-      v[h][i] = rows_gate(gv, gv) * uv;
-      amax = fmaxf(amax, finite_abs(v[h][i]));
-    }
-#pragma unroll
-  for (int x = 16; x < 16 * LANES; x *= 2) amax = fmaxf(amax, __shfl_xor(amax, x));
+  for (int i = 0; i < 8; ++i) {
+    const float gv = g[i] * (xs * sg[i]);
+    v[i] = rows_gate(gv, gv) * (u[i] * (xs * su[i]));
+    amax = fmaxf(amax, finite_abs(v[i]));
+  }
+  amax = fmaxf(amax, dppf<kDppXor1>(amax));
+  amax = fmaxf(amax, dppf<kDppXor2>(amax));
   const int z = group_exponent(amax);
   const float m = __uint_as_float((uint32_t)(127 - z) << 23);
   if (!live) return;
   uint8_t* sc = a.asc + ((n >> 7) * a.P + r) * 4 + (n >> 5 & 3);
-  if (!in) {
+  if (n >= a.N) {
     *sc = 127;
     return;
   }
-  uint32_t q[C];
 #pragma unroll
-  for (int h = 0; h < C; ++h) q[h] = pack_group4(v[h], m);
-  uint8_t* out = a.aq + r * a.N + n;
-  if (C == 4 && STRIDE == 4) {
-    st16(out, make_uint4(q[0], q[1], q[2], q[3]));
-  } else {
-#pragma unroll
-    for (int h = 0; h < C; ++h) *reinterpret_cast<uint32_t*>(out + STRIDE * h) = q[h];
-  }
+  for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], 0.f, v[i] * m);  // non-finite: NaN
+  *reinterpret_cast<uint2*>(a.aq + r * a.N + n) =
+      make_uint2(pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7]));
   *sc = (uint8_t)(z + 127);  // all lanes of a group the same
 }
+// The gate and up scales of columns n .. n + 7 of expert e.
+__device__ __forceinline__ void rows_gate_up_cols(const RowsGemm& a, int e, int n, float (&sg)[8],
+                                                  float (&su)[8]) {
+  const float* s = a.ws + (long long)e * 2 * a.N + (n < a.N ? n : 0);  // N is a multiple of 32
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sg[i] = s[i], su[i] = s[a.N + i];
+}
 
-// kRowsDown: outputs n .. n + 3 of pair row p.
-__device__ __forceinline__ void rows_down_out(const RowsGemm& a, long long p, int e, int n,
-                                              f32x4_t acc) {
-  if (n >= a.N) return;  // N is a multiple of 32
-  const float* s = a.ws + (long long)e * a.N + n;
-  *reinterpret_cast<uint2*>(a.out + p * a.N + n) = make_uint2(
-      pack_bf2_rne(acc[0] * s[0], acc[1] * s[1]), pack_bf2_rne(acc[2] * s[2], acc[3] * s[3]));
+// kRowsDown: outputs n .. n + 7 of pair row p, whose scales are ws.
+__device__ __forceinline__ void rows_down_out(const RowsGemm& a, long long p, int n,
+                                              const float (&ws)[8], const float (&v)[8]) {
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) o[i / 2] = pack_bf2_rne(v[i] * ws[i], v[i + 1] * ws[i + 1]);
+  st16(a.out + p * a.N + n, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
 // es: bytes of an element. max_tiles: entries of the tile table at most (experts), built with

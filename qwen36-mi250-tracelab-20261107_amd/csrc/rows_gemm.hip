@@ -31,7 +31,7 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
 // Few token rows: 16 NB weight rows times 16 MB token rows a workgroup, K split over its W
 // waves, operands straight from memory into the matrix instructions; the waves' sums meet in
 // LDS in a fixed order. Bound by the stream of weights.
-template <int ES, int MODE, int NB, int MB, int W, int CLASS>
+template <int ES, int MODE, int NB, int MB, int W>
 __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   __shared__ f32x4_t red[W][NB * MB][64];
   RowsTile t;
@@ -93,42 +93,49 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int m = 0; m < MB; ++m) red[wave][b * MB + m][lane] = acc[b][m];
+    for (int m = 0; m < MB; ++m) red[wave][m * NB + b][lane] = acc[b][m];
   __syncthreads();
-  auto sum = [&](int b, int m) {
-    f32x4_t s = red[0][b * MB + m][lane];
+  // Eight neighbouring outputs a thread: quads (b, 2 h) and (b, 2 h + 1) of token row (m, lr) lie 16
+  // lanes apart.
+  const int tid = threadIdx.x;
+  constexpr int PER = MODE == kRowsGateUp ? 4 : 2 * NB;  // threads of a row
+  for (int i = tid; i < 16 * MB * PER; i += W * 64) {
+    const int row = i / PER, c = i - row * PER, m = row >> 4;
+    auto sum = [&](int b, float (&v)[8]) __attribute__((always_inline)) {
+      const int l = (row & 15) + (c & 1) * 32;
+      f32x4_t s0 = red[0][m * NB + b][l], s1 = red[0][m * NB + b][l + 16];
 #pragma unroll
-    for (int w = 1; w < W; ++w) s += red[w][b * MB + m][lane];
-    return s;
-  };
-  if constexpr (MODE == kRowsGateUp) {
-    for (int m = wave; m < MB; m += W) {
-      const long long r = t.r0 + m * 16 + lr;
-      const f32x4_t g[2] = {sum(0, m), sum(1, m)}, u[2] = {sum(2, m), sum(3, m)};
-      const float xs = a.xs[a.order[min(r, t.r1 - 1)] / a.topk];
-      rows_gate_up_out<2, 4, 16>(a, r < t.r1, r, t.e, xs, blockIdx.x * 32 + 4 * kq, g, u);
+      for (int w = 1; w < W; ++w) s0 += red[w][m * NB + b][l], s1 += red[w][m * NB + b][l + 16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = s0[j], v[4 + j] = s1[j];
+    };
+    const long long r = t.r0 + row;
+    const bool live = r < t.r1;
+    const long long rr = min(r, t.r1 - 1);
+    float v[8];
+    sum(c >> 1, v);
+    if constexpr (MODE == kRowsGateUp) {
+      const int n = blockIdx.x * 32 + c * 8;
+      float u[8], sg[8], su[8];
+      sum(2 + (c >> 1), u);
+      rows_gate_up_cols(a, t.e, n, sg, su);
+      rows_gate_up_out(a, live, r, n, sg, su, a.xs[a.order[rr] / a.topk], v, u);
       // the scales behind the last group
-      const int grp = blockIdx.x + 1 + kq;
-      if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + kq < 4 && r < t.r1)
+      const int grp = blockIdx.x + 1 + c;
+      if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + c < 4 && live)
         a.asc[((grp >> 2) * a.P + r) * 4 + (grp & 3)] = 127;
-    }
-  } else {
-    for (int i = wave; i < NB * MB; i += W) {
-      const int b = i / MB, m = i - b * MB;
-      const long long r = t.r0 + m * 16 + lr;
-      const f32x4_t v = sum(b, m);
-      const int n = (blockIdx.x * NB + b) * 16 + 4 * kq;
-      if (r >= t.r1) continue;
+    } else {
+      const int n = blockIdx.x * NB * 16 + c * 8;
+      if (!live || n >= a.N) continue;
+      float ws[8];
       if (MODE == kRowsLinear) {
-        float ws[4], bias[4], o[4] = {v[0], v[1], v[2], v[3]};
+        float bias[8];
         rows_linear_cols(a, n, ws, bias);
-        const float xs = a.xs ? a.xs[r] : 1.f;
-        if (a.N % 4 == 0)
-          rows_linear_out<CLASS, 4, true>(a, r, n, xs, ws, bias, o);
-        else
-          rows_linear_out<CLASS, 4, false>(a, r, n, xs, ws, bias, o);
+        rows_linear_out(a, r, n, a.xs ? a.xs[r] : 1.f, ws, bias, v);
       } else {
-        rows_down_out(a, a.order[r], t.e, n, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ws[j] = a.ws[(long long)t.e * a.N + n + j];
+        rows_down_out(a, a.order[r], n, ws, v);
       }
     }
   }
@@ -149,28 +156,50 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // ends with 4 NA neighbouring outputs (2 NA gate and 2 NA up ones, half a group of 32) of each token
 // and stores them in 16-byte pieces.
 //
-// A step's products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0), each
-// reading from LDS, between its matrix instructions, the half that the next one needs; the last two
-// read the next step's first halves, the tokens' into the registers that held half 1. One barrier a
-// step, after the second quarter: the step has been read by all, and the next one has arrived.
+// A step's products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0). Between
+// its matrix instructions, which leave three of four issue slots free, each reads from LDS, early, the
+// half that the next one needs, and the last two issue the DMA loads; they read the next step's
+// first halves, the tokens' into the registers that held half 1. One barrier a step, after the second
+// quarter: the step has been read by all, and the next one has arrived. (With the loads issued
+// together after the barrier and the reads after each block's products, a step of 256 x 256
+// took 4400 cycles; its products take 2048.)
 struct Frag {
   u32x4v v[2];
 };
-template <int ES, bool SC>
-__device__ __forceinline__ f32x4_t tile_mma(const Frag& w, const Frag& t, uint32_t sb, f32x4_t c) {
-  const uint4 w0 = __builtin_bit_cast(uint4, w.v[0]), w1 = __builtin_bit_cast(uint4, w.v[1]);
-  const uint4 t0 = __builtin_bit_cast(uint4, t.v[0]), t1 = __builtin_bit_cast(uint4, t.v[1]);
-  return SC ? rows_mma_scaled(w0, w1, t0, t1, (int)sb, c) : rows_mma<ES>(w0, w1, t0, t1, c);
+// acc += w . t for one step (bf16: for its half H), in place: as asm, because the compiler, given 256
+// sums, moves some of them between registers around every product. It does not see these writes,
+// so the sums are read only behind mma_done.
+template <int ES, bool SC, int H>
+__device__ __forceinline__ void tile_mma(const Frag& w, const Frag& t, uint32_t sb, f32x4_t& acc) {
+  if constexpr (ES == 2) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(w.v[H]), "v"(t.v[H]));
+  } else {
+    typedef unsigned u32x8v __attribute__((ext_vector_type(8)));
+    const u32x8v w8 = __builtin_shufflevector(w.v[0], w.v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    const u32x8v t8 = __builtin_shufflevector(t.v[0], t.v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    if constexpr (SC) {
+      const uint32_t one = 0x7f;
+      asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                   : "+a"(acc) : "v"(w8), "v"(t8), "v"(one), "v"(sb));
+    } else {
+      asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(acc) : "v"(w8), "v"(t8));
+    }
+  }
 }
-__device__ __forceinline__ u32x4v lds_read16(uint32_t addr) {
-  u32x4v r;
-  asm volatile("ds_read_b128 %0, %1" : "=v"(r) : "v"(addr));
-  return r;
-}
+// The last product's passes, before anything else reads the sums.
+__device__ __forceinline__ void mma_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+template <int OFF>
 __device__ __forceinline__ uint32_t lds_read4(uint32_t addr) {
   uint32_t r;
-  asm volatile("ds_read_b32 %0, %1" : "=v"(r) : "v"(addr));
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF));
   return r;
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (N > 0) {
+    static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
 }
 __device__ __forceinline__ void dma4_buffer(__amdgpu_buffer_rsrc_t buf, void* lds, uint32_t voff,
                                             uint32_t soff) {
@@ -190,7 +219,7 @@ struct TileShape {
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
-template <int ES, int MODE, int NA, int NB, int CLASS, bool VEC>
+template <int ES, int MODE, int NA, int NB>
 __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int ntile) {
   using S = TileShape<MODE, NA, NB>;
   constexpr bool SC = S::kScaled;
@@ -232,10 +261,9 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   const int n0 = col * S::kOut;
   const uint32_t ldw = (uint32_t)a.ldw, ldx = (uint32_t)a.ldx;
   const int wrows = MODE == kRowsGateUp ? 2 * a.N - n0 : min(S::kWRows, a.N - n0);
-  // (a load's uniform offset never passes its buffer's end, its lanes' own offsets may)
-  const uint32_t wbytes = (uint32_t)(wrows - 1) * ldw + a.Kb;
   const __amdgpu_buffer_rsrc_t wbuf = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(a.w + t.e * a.estride + (long long)n0 * a.ldw), 0, wbytes, 0x00020000);
+      const_cast<uint8_t*>(a.w + t.e * a.estride + (long long)n0 * a.ldw), 0,
+      (uint32_t)(wrows - 1) * ldw + a.Kb, 0x00020000);
   uint32_t wunit[2], woff[2];  // by load parity (the key of row0 + 32)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -261,65 +289,78 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   const __amdgpu_buffer_rsrc_t sbuf = __builtin_amdgcn_make_buffer_rsrc(
       SC ? a.asc + t.r0 * 4 : nullptr, 0,
       SC ? (uint32_t)(((a.Kb + 127) / 128 - 1) * a.P * 4 + ntok * 4) : 0, 0x00020000);
+  // (the last wave's scale load, past the stage's rows, repeats the one before)
+  const int srow = min(wave, S::kTRows / 64 - 1) * 64;
+  const uint32_t soff = srow + lane < ntok ? (srow + lane) * 4 : kNowhere;
   const int nd = (a.Kb + 127) / 128;
-  const bool ragged = a.Kb % 128 != 0;
-  auto issue_a = [&](int d) __attribute__((always_inline)) {
-    char* st = lds + (d % S::kSA) * S::kAStage;
-    const uint32_t k0 = d * 128;
-    const bool last = ragged && d == nd - 1;
+  // The loads of step d; past the last one, of nothing, so that every step has the same loads in
+  // flight. A load's uniform offset never passes its buffer's end: the rows of a group past the last
+  // row are those of the first group again. All of it is selects and sums: a branch among the
+  // products would cost more than they do.
+  uint32_t wrow[LA], xrow[LB];
 #pragma unroll
-    for (int i = 0; i < LA; ++i) {
-      uint32_t soff = k0;
-      if (MODE == kRowsGateUp)  // LDS rows: per wm 8 NA gate rows, then their up rows
-        soff += (uint32_t)(((i / (NA / 4)) & 1) * a.N + (i / (NA / 2)) * 8 * NA +
-                           (i % (NA / 4)) * 32) * ldw;
-      else
-        soff += 32u * i * ldw;
-      const bool past = last && k0 + wunit[i & 1] >= (uint32_t)a.Kb;
-      const bool in = soff - k0 < wbytes;  // else all of its rows are past the last one
-      dma16_buffer(wbuf, st + (wave + 4 * i) * 1024, past || !in ? kNowhere : woff[i & 1], in ? soff : 0);
-    }
-  };
-  auto issue_b = [&](int d) __attribute__((always_inline)) {
-    char* st = lds + S::kSA * S::kAStage + (d % S::kSB) * S::kBStage;
-    const uint32_t k0 = d * 128;
-    const bool past = ragged && d == nd - 1 && k0 + tunit >= (uint32_t)a.Kb;
+  for (int i = 0; i < LA; ++i) {
+    // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows
+    const uint32_t r = MODE == kRowsGateUp ? (uint32_t)(((i / (NA / 4)) & 1) * a.N +
+                                                        (i / (NA / 2)) * 8 * NA + (i % (NA / 4)) * 32)
+                                           : 32u * i;
+    wrow[i] = __builtin_amdgcn_readfirstlane((int)r < wrows ? r * ldw : 0);
+  }
 #pragma unroll
-    for (int i = 0; i < LB; ++i) {
-      const uint32_t v = MODE == kRowsGateUp ? toff[i] : toff[0];
-      const bool in = MODE == kRowsGateUp || 32 * i < ntok;
-      const uint32_t soff = MODE == kRowsGateUp ? k0 : in ? k0 + 32u * i * ldx : 0;
-      dma16_buffer(xbuf, st + (wave + 4 * i) * 1024, past || !in ? kNowhere : v, soff);
-    }
-    if (SC && wave < S::kTRows / 64)  // a dword of four groups' scales per row
-      dma4_buffer(sbuf, st + S::kTRows * 128 + wave * 256,
-                  wave * 64 + lane < ntok ? (wave * 64 + lane) * 4 : kNowhere,
-                  (uint32_t)(d * a.P * 4));
+  for (int i = 0; i < LB; ++i)
+    xrow[i] = __builtin_amdgcn_readfirstlane(MODE != kRowsGateUp && 32 * i < ntok ? 32u * i * ldx : 0);
+  struct Step {
+    uint32_t k0, stage;  // byte of K, LDS offset of the stage
+    uint32_t off[2];     // kNowhere for the lanes past the row's end, else 0
   };
+  auto past = [&](int d, uint32_t unit) __attribute__((always_inline)) {
+    return (uint32_t)d * 128 + unit < (uint32_t)a.Kb ? 0u : kNowhere;
+  };
+  auto step_a = [&](int d, uint32_t stage) __attribute__((always_inline)) {
+    return Step{(uint32_t)min(d, nd - 1) * 128, stage, {past(d, wunit[0]), past(d, wunit[1])}};
+  };
+  auto step_b = [&](int d, uint32_t stage) __attribute__((always_inline)) {
+    return Step{(uint32_t)min(d, nd - 1) * 128, stage, {past(d, tunit), d < nd ? 0u : kNowhere}};
+  };
+  auto load_a = [&](const Step& st, auto ic) __attribute__((always_inline)) {
+    constexpr int i = decltype(ic)::value;
+    dma16_buffer(wbuf, lds + st.stage + (wave + 4 * i) * 1024, woff[i & 1] | st.off[i & 1],
+                 st.k0 + wrow[i]);
+  };
+  auto load_b = [&](const Step& st, auto ic) __attribute__((always_inline)) {
+    constexpr int i = decltype(ic)::value;
+    if constexpr (i == LB)  // a dword of four groups' scales per row
+      dma4_buffer(sbuf, lds + st.stage + S::kTRows * 128 + srow * 4, soff | st.off[1],
+                  (st.k0 >> 7) * (uint32_t)(a.P * 4));
+    else
+      dma16_buffer(xbuf, lds + st.stage + (wave + 4 * i) * 1024,
+                   toff[MODE == kRowsGateUp ? i : 0] | st.off[0], st.k0 + xrow[i]);
+  };
+  constexpr int NLB = LB + (SC ? 1 : 0);
+  constexpr int kB0 = S::kSA * S::kAStage;  // the token ring
 
-  // ---- fragment addresses
+  // ---- fragments
   const uint32_t lbase = lds_addr(lds);
   uint32_t aaddr, baddr;
   {
     const int r = wm * 16 * NA + (lr >> 2) * SPAN + (lr & 3);  // block b: + 4 b rows
     const int key = (r & 3) | (((r / SPAN) & 1) << 2);
     aaddr = lbase + r * 128 + (kq ^ key) * 16;
-    baddr = lbase + S::kSA * S::kAStage + (wn * 16 + lr) * 128 + (kq ^ (lr & 7)) * 16;
+    baddr = lbase + (wn * 16 + lr) * 128 + (kq ^ (lr & 7)) * 16;
   }
-  const uint32_t saddr = lbase + S::kSA * S::kAStage + S::kTRows * 128 + (wn * 16 + lr) * 4;
+  const uint32_t saddr = lbase + S::kTRows * 128 + (wn * 16 + lr) * 4;
   // weight block b: gate blocks first (kRowsGateUp), then the up blocks 8 NA rows on
-  auto read_a = [&](int d, int b, Frag& f) __attribute__((always_inline)) {
-    const uint32_t at = aaddr + (d % S::kSA) * S::kAStage +
-                        (MODE == kRowsGateUp && b >= HA ? 8 * NA + 4 * (b - HA) : 4 * b) * 128;
-    f.v[0] = lds_read16(at);
-    f.v[1] = lds_read16(at ^ 64);
+  auto read_a = [&](uint32_t at, auto bc, Frag& f) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+    constexpr int off = (MODE == kRowsGateUp && b >= HA ? 8 * NA + 4 * (b - HA) : 4 * b) * 128;
+    f.v[0] = lds_read_frag<off>(at);
+    f.v[1] = lds_read_frag<off>(at ^ 64);
   };
-  auto read_b = [&](int d, int b, Frag& f, uint32_t& sc) __attribute__((always_inline)) {
-    const uint32_t st = (d % S::kSB) * S::kBStage;
-    const uint32_t at = baddr + st + b * 32 * 128;
-    f.v[0] = lds_read16(at);
-    f.v[1] = lds_read16(at ^ 64);
-    if (SC) sc = lds_read4(saddr + st + b * 32 * 4);
+  auto read_b = [&](uint32_t stage, auto bc, Frag& f, uint32_t& sc) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+    f.v[0] = lds_read_frag<b * 32 * 128>(baddr + stage);
+    f.v[1] = lds_read_frag<b * 32 * 128>((baddr + stage) ^ 64);
+    if constexpr (SC) sc = lds_read4<b * 32 * 4>(saddr + stage);
   };
 
   f32x4_t acc[NA][NB];
@@ -345,127 +386,167 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
         sc[i] >>= 8 * kq;
       }
     }
+    if (SC) asm volatile("s_nop 3");  // before a product reads them
   };
-  // One quarter: weight half x, token half y; work(i) is called after token block i's products.
+  // One quarter: weight half x, token half y. After its product p (bf16: all first halves, then all
+  // second ones, so that no product waits for the one before), what falls due: read k of NR at
+  // product RS k, load k of NL at product (k PROD) / NL (one later where there is room).
+  constexpr int PROD = HA * HB * ES;
   auto quarter = [&](const Frag (&w)[HA], const Frag (&tk)[HB], const uint32_t (&sc)[HB], auto xh, auto yh,
-                     auto work) __attribute__((always_inline)) {
+                     auto nr, auto read, auto nl, auto load) __attribute__((always_inline)) {
     constexpr int X = decltype(xh)::value, Y = decltype(yh)::value;
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      if (Y * HB + i < nb) {
-#pragma unroll
-        for (int j = 0; j < HA; ++j)
-          acc[X * HA + j][Y * HB + i] =
-              tile_mma<ES, SC>(w[j], tk[i], sc[i], acc[X * HA + j][Y * HB + i]);
-      }
+    constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value;
+    constexpr int RS = PROD / 2 / NR > 0 ? PROD / 2 / NR : 1;
+    constexpr int LO = NL > 0 && PROD / (NL > 0 ? NL : 1) > 1 ? 1 : 0;
+    static_for<PROD>([&](auto prod) __attribute__((always_inline)) {
+      constexpr int p = decltype(prod)::value, H = p / (HA * HB), i = p / HA % HB, j = p % HA;
+      tile_mma<ES, SC, H>(w[j], tk[i], sc[i], acc[X * HA + j][Y * HB + i]);
       __builtin_amdgcn_sched_barrier(0);
-      work(i);
+      static_for<NR>([&](auto k) __attribute__((always_inline)) {
+        if constexpr ((decltype(k)::value * RS < PROD ? decltype(k)::value * RS : PROD - 1) == p) read(k);
+      });
+      static_for<NL>([&](auto k) __attribute__((always_inline)) {
+        if constexpr (decltype(k)::value * PROD / NL + LO == p) load(k);
+      });
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
   };
-  const std::integral_constant<int, 0> c0{};
-  const std::integral_constant<int, 1> c1{};
+  using std::integral_constant;
+  const integral_constant<int, 0> c0{};
+  const integral_constant<int, 1> c1{};
+  const integral_constant<int, HA> cha{};
+  const integral_constant<int, HB> chb{};
+  const auto none = [](auto) {};
+  // Ring offsets: the stages of this step and the next ones.
+  uint32_t ra[3] = {0, S::kAStage, 2 * S::kAStage}, rb[2] = {kB0, kB0 + S::kBStage};
   // Step d with its tokens' half 0 in p; half 1 goes to q, and the next step's half 0 after it.
   auto step = [&](int d, Frag (&p)[HB], uint32_t (&sp)[HB], Frag (&q)[HB], uint32_t (&sq)[HB])
                   __attribute__((always_inline)) {
-    quarter(a0, p, sp, c0, c0, [&](int i) __attribute__((always_inline)) { read_b(d, HB + i, q[i], sq[i]); });
+    const uint32_t at = aaddr + ra[0], at1 = aaddr + ra[1];
+    quarter(a0, p, sp, c0, c0, chb, [&](auto k) __attribute__((always_inline)) {
+      constexpr int K = decltype(k)::value;
+      read_b(rb[0], integral_constant<int, HB + K>{}, q[K], sq[K]);
+    }, c0, none);
     lds_frags_ready();
     ready_b(q, sq);
-    quarter(a0, q, sq, c0, c1, [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = i * HA / HB; j < (i + 1) * HA / HB; ++j) read_a(d, HA + j, a1[j]);
-    });
+    quarter(a0, q, sq, c0, c1, cha, [&](auto k) __attribute__((always_inline)) {
+      constexpr int K = decltype(k)::value;
+      read_a(at, integral_constant<int, HA + K>{}, a1[K]);
+    }, c0, none);
     lds_frags_ready();
     ready_a(a1);
-    wait_loads(d + 2 < nd ? LA : 0);
+    wait_loads(LA);  // step d + 2's weights may be in flight
     __builtin_amdgcn_s_barrier();
-    if (d + 2 < nd) issue_b(d + 2);
-    if (d + 3 < nd) issue_a(d + 3);
-    quarter(a1, q, sq, c1, c1, [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = i * HA / HB; j < (i + 1) * HA / HB; ++j) read_a(d + 1, j, a0[j]);
-    });
-    quarter(a1, p, sp, c1, c0, [&](int i) __attribute__((always_inline)) { read_b(d + 1, i, q[i], sq[i]); });
+    const Step nb2 = step_b(d + 2, rb[0]), na3 = step_a(d + 3, ra[0]);
+    quarter(a1, q, sq, c1, c1, cha, [&](auto k) __attribute__((always_inline)) {
+      read_a(at1, k, a0[decltype(k)::value]);
+    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb2, k); });
+    quarter(a1, p, sp, c1, c0, chb, [&](auto k) __attribute__((always_inline)) {
+      constexpr int K = decltype(k)::value;
+      read_b(rb[1], k, q[K], sq[K]);
+    }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na3, k); });
     lds_frags_ready();
     ready_a(a0);
     ready_b(q, sq);
+    const uint32_t t0 = ra[0], u0 = rb[0];
+    ra[0] = ra[1], ra[1] = ra[2], ra[2] = t0;
+    rb[0] = rb[1], rb[1] = u0;
   };
-  issue_a(0);
-  issue_b(0);
-  if (nd > 1) issue_a(1);
-  if (nd > 1) issue_b(1);
-  if (nd > 2) issue_a(2);
-  const int lb = LB + (SC && wave < S::kTRows / 64 ? 1 : 0);
-  wait_loads((LA + lb) * (nd > 1) + LA * (nd > 2));
+  // (in the order in which the steps issue them: tokens, then weights one further on)
+  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(0, ra[0]), k); });
+  static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(0, rb[0]), k); });
+  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(1, ra[1]), k); });
+  static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(1, rb[1]), k); });
+  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(2, ra[2]), k); });
+  wait_loads(2 * LA + NLB);  // step 0 has arrived
   __builtin_amdgcn_s_barrier();
-#pragma unroll
-  for (int j = 0; j < HA; ++j) read_a(0, j, a0[j]);
-#pragma unroll
-  for (int i = 0; i < HB; ++i) read_b(0, i, bx[i], sx[i]);
+  static_for<HA>([&](auto k) __attribute__((always_inline)) { read_a(aaddr, k, a0[decltype(k)::value]); });
+  static_for<HB>([&](auto k) __attribute__((always_inline)) {
+    constexpr int K = decltype(k)::value;
+    read_b(kB0, k, bx[K], sx[K]);
+  });
   lds_frags_ready();
   ready_a(a0);
   ready_b(bx, sx);
   for (int d = 0; d < nd; d += 2) {
     step(d, bx, sx, by, sy);
-    if (d + 1 >= nd) break;
-    step(d + 1, by, sy, bx, sx);
+    step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
   }
+  wait_loads(0);
+  mma_done();
 
-  // ---- epilogue
-  const int ncols = n0 + wm * (S::kOut / 2) + kq * SPAN;  // the lane's first output
-  if constexpr (MODE == kRowsLinear) {
-    float xs[NB];
+  // ---- epilogue: half of the wave's token blocks at a time through LDS, row by row, so that one small
+  // loop serves all of the sums (unrolled over the registers it was 80 KB of instructions, which took
+  // longer to fetch than a tile of K = 1024 to multiply) and a row's outputs are stored together
+  constexpr int kStride = 16 * NA + 4;  // floats of a row: 16 bytes on, so that eight rows differ in banks
+  static_assert(4 * HB * 16 * kStride * 4 <= S::kLds, "the waves' parts");
+  constexpr int PER = (MODE == kRowsGateUp ? NA : 2 * NA);  // lanes of a row, eight outputs each
+  constexpr int RPI = 64 / PER;
+  float* part = reinterpret_cast<float*>(lds) + wave * HB * 16 * kStride;
+  const int c = lane % PER, rsub = lane / PER;
+  const int n = n0 + wm * (S::kOut / 2) + c * 8;
+  float ws[8], other[8];  // scales, and the up scales or the bias
+  if constexpr (MODE == kRowsGateUp)
+    rows_gate_up_cols(a, t.e, n, ws, other);
+  else if constexpr (MODE == kRowsLinear)
+    rows_linear_cols(a, n, ws, other);
+  else
 #pragma unroll
-    for (int b = 0; b < NB; ++b) xs[b] = a.xs ? a.xs[min(t.r0 + (2 * b + wn) * 16 + lr, t.r1 - 1)] : 1.f;
+    for (int i = 0; i < 8; ++i) ws[i] = a.ws[(long long)t.e * a.N + min(n + i, a.N - 1)];
+  __syncthreads();  // the stages have been read
 #pragma unroll
-    for (int x = 0; x < NA; x += 2) {
-      float ws[8], bias[8];
-      rows_linear_cols(a, ncols + 4 * x, ws, bias);
+  for (int half = 0; half < 2; ++half) {
+    const int blocks = min(HB, nb - half * HB);
+    if (blocks <= 0) break;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const long long r = t.r0 + (2 * b + wn) * 16 + lr;
-        __builtin_amdgcn_sched_barrier(0);  // one unit's values live at a time
-        if (r >= t.r1) continue;
-        const f32x4_t u = acc[x][b], w = acc[x + 1][b];
-        float o[8] = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
-        rows_linear_out<CLASS, 8, VEC>(a, r, ncols + 4 * x, xs[b], ws, bias, o);
+    for (int i = 0; i < HB; ++i)
+#pragma unroll
+      for (int x = 0; x < NA; ++x) {
+        const int col = MODE == kRowsGateUp && x >= HA ? 8 * NA + kq * SPAN + 4 * (x - HA)
+                                                       : kq * SPAN + 4 * x;
+        *reinterpret_cast<f32x4_t*>(part + (i * 16 + lr) * kStride + col) = acc[x][half * HB + i];
       }
-    }
-  } else {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses run in order)
+    for (int row = rsub; row < blocks * 16; row += RPI) {
+      const long long r = t.r0 + (2 * (half * HB + (row >> 4)) + wn) * 16 + (row & 15);
+      const float* src = part + row * kStride + c * 8;
+      float v[8];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if (b >= nb) break;
-      const long long r = t.r0 + (2 * b + wn) * 16 + lr;
+      for (int j = 0; j < 8; ++j) v[j] = src[j];
       const bool live = r < t.r1;
       if constexpr (MODE == kRowsGateUp) {
-        f32x4_t g[HA], u[HA];
+        float u[8];
 #pragma unroll
-        for (int x = 0; x < HA; ++x) g[x] = acc[x][b], u[x] = acc[HA + x][b];
+        for (int j = 0; j < 8; ++j) u[j] = src[8 * NA + j];
         const float xs = a.xs[a.order[min(r, t.r1 - 1)] / a.topk];
-        rows_gate_up_out<HA, 32 / SPAN, 4>(a, live, r, t.e, xs, ncols, g, u);
-      } else if (live) {
-        const long long p = a.order[r];
-#pragma unroll
-        for (int x = 0; x < NA; ++x) rows_down_out(a, p, t.e, ncols + 4 * x, acc[x][b]);
+        rows_gate_up_out(a, live, r, n, ws, other, xs, v, u);
+      } else if (live && n < a.N) {
+        if constexpr (MODE == kRowsLinear)
+          rows_linear_out(a, r, n, a.xs ? a.xs[r] : 1.f, ws, other, v);
+        else
+          rows_down_out(a, a.order[r], n, ws, v);
       }
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-template <int ES, int MODE, int MB, int CLASS = 0>
+template <int ES, int MODE, int MB>
 hipError_t launch_few(const RowsGemm& a, hipStream_t s) {
   constexpr int NB = MODE == kRowsGateUp ? 4 : 2, W = 4;
   const long long cols = MODE == kRowsGateUp ? a.N / 32 : (a.N + 16 * NB - 1) / (16 * NB);
   const long long tiles = MODE == kRowsLinear ? (a.M + 16 * MB - 1) / (16 * MB) : a.MT;
   if (tiles <= 0 || cols <= 0) return hipSuccess;
   if (tiles > 65535 || cols > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W, CLASS>), dim3((unsigned)cols, (unsigned)tiles),
+  hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W>), dim3((unsigned)cols, (unsigned)tiles),
                      dim3(W * 64), 0, s, a);
   return hipGetLastError();
 }
 
 // A kernel's dynamic LDS above the default limit, allowed once per device.
-template <int ES, int MODE, int NA, int NB, int CLASS, bool VEC>
+template <int ES, int MODE, int NA, int NB>
 hipError_t allow_tile_lds() {
   static std::mutex mu;
   static uint64_t done = 0;  // bit d: device d
@@ -475,14 +556,14 @@ hipError_t allow_tile_lds() {
   if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(mu);
   if (done >> dev & 1) return hipSuccess;
-  err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_tile<ES, MODE, NA, NB, CLASS, VEC>),
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_tile<ES, MODE, NA, NB>),
                             hipFuncAttributeMaxDynamicSharedMemorySize,
                             TileShape<MODE, NA, NB>::kLds);
   if (err == hipSuccess) done |= uint64_t(1) << dev;
   return err;
 }
 
-template <int ES, int MODE, int NA, int NB, int CLASS = 0, bool VEC = true>
+template <int ES, int MODE, int NA, int NB>
 hipError_t launch_tile(const RowsGemm& a, hipStream_t s) {
   using S = TileShape<MODE, NA, NB>;
   const long long ncol = (a.N + S::kOut - 1) / S::kOut;
@@ -490,9 +571,9 @@ hipError_t launch_tile(const RowsGemm& a, hipStream_t s) {
   if (ntile <= 0) return hipSuccess;
   const long long grid = MODE == kRowsLinear ? (ncol * ntile + 7) / 8 * 8 : (ntile + 7) / 8 * 8 * ncol;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipError_t err = allow_tile_lds<ES, MODE, NA, NB, CLASS, VEC>();
+  hipError_t err = allow_tile_lds<ES, MODE, NA, NB>();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL((k_rows_tile<ES, MODE, NA, NB, CLASS, VEC>), dim3((unsigned)grid), dim3(256), S::kLds, s, a,
+  hipLaunchKernelGGL((k_rows_tile<ES, MODE, NA, NB>), dim3((unsigned)grid), dim3(256), S::kLds, s, a,
                      (int)ncol, (int)ntile);
   return hipGetLastError();
 }
@@ -507,16 +588,12 @@ bool tile_fits(RowsMode mode, const RowsGemm& a) {
   return true;
 }
 
-template <int ES, int CLASS>
-hipError_t launch_linear(const RowsGemm& a, int c, bool vec, hipStream_t s) {
-  if (c == 256) return launch_tile<ES, kRowsLinear, 8, 8, CLASS, true>(a, s);
-  if (c == 128)
-    return vec ? launch_tile<ES, kRowsLinear, 4, 4, CLASS, true>(a, s)
-               : launch_tile<ES, kRowsLinear, 4, 4, CLASS, false>(a, s);
-  if (c == 64)
-    return vec ? launch_tile<ES, kRowsLinear, 2, 2, CLASS, true>(a, s)
-               : launch_tile<ES, kRowsLinear, 2, 2, CLASS, false>(a, s);
-  return c ? launch_few<ES, kRowsLinear, 4, CLASS>(a, s) : launch_few<ES, kRowsLinear, 1, CLASS>(a, s);
+template <int ES>
+hipError_t launch_linear(const RowsGemm& a, int c, hipStream_t s) {
+  if (c == 256) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
+  if (c == 128) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
+  if (c == 64) return launch_tile<ES, kRowsLinear, 2, 2>(a, s);
+  return c ? launch_few<ES, kRowsLinear, 4>(a, s) : launch_few<ES, kRowsLinear, 1>(a, s);
 }
 
 }  // namespace
@@ -539,14 +616,7 @@ hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_r
       c = n(256) >= 200 ? 256 : n(128) >= 128 ? 128 : 64;
     }
     if (!tile_fits(mode, a) && c > 1) c = 1;
-    const bool vec = a.N % 8 == 0;
-    if (c == 256 && !vec) c = 128;
-    switch (rows_act_class(a.act)) {
-#define L(CLASS) \
-  case CLASS: return es == 2 ? launch_linear<2, CLASS>(a, c, vec, s) : launch_linear<1, CLASS>(a, c, vec, s);
-      L(kClassLinear) L(kClassGate) L(kClassErf)
-#undef L
-    }
+    return es == 2 ? launch_linear<2>(a, c, s) : launch_linear<1>(a, c, s);
   }
   if (es != 1 || a.N % 32) return hipErrorInvalidValue;
   if (mode == kRowsGateUp) {
