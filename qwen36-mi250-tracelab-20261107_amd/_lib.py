@@ -136,8 +136,9 @@ def ptr(t) -> int | None:
 
 
 def stream_of(t) -> int:
-    """The current HIP stream of ``t``'s device, as the C ABI's ``void* stream``."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current HIP stream of ``t``'s device, as the C ABI's ``void* stream`` (0.1 µs; building
+    a ``torch.cuda.Stream`` for it takes 3)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 _WORKSPACES: dict = {}

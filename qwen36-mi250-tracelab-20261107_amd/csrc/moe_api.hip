@@ -1179,18 +1179,19 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
   CHECK_ARG(x && w && out, "linear: null pointer");
   CHECK_ARG((es == 1) == (x_scale != nullptr) && (es == 1) == (w_scale != nullptr),
             "linear: e4m3 operands take x_scale and w_scale, bf16 ones neither");
-  CHECK_ARG(ldx >= K && ldw >= K && ldx * es % 16 == 0 && ldw * es % 16 == 0 &&
-                ((uintptr_t)x | (uintptr_t)w) % 16 == 0,
-            "linear: rows of x and w must start at multiples of 16 bytes, ldx and ldw >= K");
-  CHECK_ARG((((uintptr_t)out | (uintptr_t)mul | (uintptr_t)residual) % 16) == 0 &&
-                (uintptr_t)bias % (bias_f32 ? 4 : 2) == 0,
-            "linear: out, mul and residual must be 16-byte aligned, bias as its type");
+  CHECK_ARG(ldx >= K && ldw >= K && ldx * es <= (1 << 22) && ldw * es <= (1 << 22),
+            "linear: ldx and ldw must be >= K and at most 4 MiB");
   const long long n = 2LL * M * N;
   const Span in[] = {{x, ((M - 1) * ldx + K) * es}, {w, ((N - 1) * ldw + K) * es},
                      {x_scale, 4LL * M}, {w_scale, 4LL * N}, {bias, (bias_f32 ? 4LL : 2LL) * N},
                      {mul, n}, {residual, n}};
   const Span o{out, n};
   CHECK_ARG(apart(in, 7, &o, 1), "linear: out must not overlap the inputs");
+  CHECK_ARG(ldx * es % 16 == 0 && ldw * es % 16 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0,
+            "linear: rows of x and w must start at multiples of 16 bytes (ldx %lld, ldw %lld)", ldx, ldw);
+  CHECK_ARG((((uintptr_t)out | (uintptr_t)mul | (uintptr_t)residual) % 16) == 0 &&
+                (uintptr_t)bias % (bias_f32 ? 4 : 2) == 0,
+            "linear: out, mul and residual must be 16-byte aligned, bias as its type");
   RowsGemm a{};
   a.x = static_cast<const uint8_t*>(x), a.ldx = ldx * es;
   a.w = static_cast<const uint8_t*>(w), a.ldw = ldw * es;

@@ -418,46 +418,58 @@ def add_rms(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, eps: 
 
 
 # ------------------------------------------------------------------------- 8-bit activations
+#
+# These are called per layer and token, so their checks are the few plain comparisons below: a call
+# of the smallest size costs 6 to 8 µs on the host, of which the launch and the outputs'
+# allocations are 5.
 
 
-def _same_device(first: torch.Tensor, **others) -> None:
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, the input on {first.device}")
+def _input(t: torch.Tensor, dtype: torch.dtype, name: str, dev: int | None = None) -> torch.Tensor:
+    """``t`` contiguous at a multiple of 16 bytes (a view into a larger tensor may not be), of
+    ``dtype`` and on device ``dev``."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype} (got {t.dtype})")
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the input on cuda:{dev}")
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
-def _call(name: str, device: torch.device, fn, *args) -> None:
-    """``fn(*args, stream)`` with ``device`` current: a launch goes to the current device."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
-        return
-    with torch.cuda.device(device):
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+def _vector(t: torch.Tensor | None, dtypes: tuple, name: str, n: int, dev: int) -> torch.Tensor:
+    if t is None or t.dtype not in dtypes or t.numel() != n or t.get_device() != dev:
+        kind = " or ".join(str(d) for d in dtypes)
+        raise ValueError(f"{name} must be {n} {kind} values on cuda:{dev}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous, at a multiple of 16 bytes (a view into a larger tensor may not be)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _call(name: str, dev: int, fn, *args) -> None:
+    """``fn(*args, stream)`` with device ``dev`` current: a launch goes to the current device."""
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, name)
 
 
-def _scales(t, name: str, n: int) -> torch.Tensor:
-    if t is None or t.dtype != torch.float32 or t.numel() != n:
-        raise ValueError(f"{name} must be {n} float32 values")
-    return t.contiguous()
+_F32 = (torch.float32,)
+_BIAS = (torch.bfloat16, torch.float32)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(q float8_e4m3fn [..., n], scale fp32 [...]) of ``x`` [..., n] bf16: per row
-    scale = amax / 448 over the finite values (1 for a row of zeros; amax counts as 2^-100 at
-    least) and q = e4m3(x / scale), ties to even. NaN and infinite values become NaN. The format
-    of ``fp8.quantize_rows``, for activations."""
-    _need_cuda(x)
-    x2 = _aligned(_bf16(x, "x").reshape(-1, x.shape[-1]))
-    rows, n = x2.shape
-    q = torch.empty(x.shape, dtype=FP8, device=x.device)
+    """(q float8_e4m3fn [..., n], scale fp32 [...]) of ``x`` [..., n] bf16, n a multiple of 8 up
+    to 8192: per row scale = amax / 448 over the finite values (1 for a row of zeros; amax counts
+    as 2^-100 at least) and q = e4m3(x / scale), ties to even. NaN and infinite values become NaN.
+    The format of ``fp8.quantize_rows``, for activations."""
+    x = _input(x, torch.bfloat16, "x")
+    n, dev = x.shape[-1], x.get_device()
+    q = torch.empty_like(x, dtype=FP8)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call("quantize_rows", x.device, _lib.load().moe_quantize_rows, x2.data_ptr(), rows, n,
+    _call("quantize_rows", dev, _lib.load().moe_quantize_rows, x.data_ptr(), scale.numel(), n,
           q.data_ptr(), scale.data_ptr())
     return q, scale
 
@@ -466,25 +478,25 @@ def add_rms_fp8(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, e
                 return_norm: bool = False):
     """``add_rms`` with the norm in 8 bits: (total, q, scale), and with ``return_norm`` the
     bf16 norm as a fourth item (what a bf16 router reads). q and scale are ``quantize_rows`` of
-    the fp32 norm: it is rounded once, not to bf16 first."""
-    _need_cuda(x, h, weight)
-    _same_device(x, h=h, weight=weight)
-    x2 = _aligned(_bf16(x, "x").reshape(-1, x.shape[-1]))
-    rows, n = x2.shape
-    if h is not None and h.shape != x.shape:
-        raise ValueError(f"h has shape {tuple(h.shape)}, x {tuple(x.shape)}")
-    h2 = None if h is None else _aligned(_bf16(h, "h"))
-    w = _aligned(_bf16(weight, "weight"))
-    if w.numel() != n:
-        raise ValueError(f"weight must have {n} elements (got {w.numel()})")
-    total = x2 if h2 is None else torch.empty_like(x2)
-    q = torch.empty(x.shape, dtype=FP8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    norm = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if return_norm else None
-    _call("add_rms_fp8", x.device, _lib.load().moe_add_rmsnorm_fp8, x2.data_ptr(), ptr(h2),
-          w.data_ptr(), rows, n, float(eps), None if h2 is None else total.data_ptr(),
-          q.data_ptr(), scale.data_ptr(), ptr(norm))
-    total = total.view(x.shape)
+    the fp32 norm: it is rounded once, not to bf16 first. With ``h`` None total is ``x``."""
+    x = _input(x, torch.bfloat16, "x")
+    shape, dev = x.shape, x.get_device()
+    n = shape[-1]
+    weight = _input(weight, torch.bfloat16, "weight", dev)
+    if weight.numel() != n:
+        raise ValueError(f"weight must have {n} elements (got {weight.numel()})")
+    total, added = x, None
+    if h is not None:
+        if h.shape != shape:
+            raise ValueError(f"h has shape {tuple(h.shape)}, x {tuple(shape)}")
+        h = _input(h, torch.bfloat16, "h", dev)
+        total = torch.empty_like(x)
+        added = total.data_ptr()
+    q = torch.empty_like(x, dtype=FP8)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    norm = torch.empty_like(x) if return_norm else None
+    _call("add_rms_fp8", dev, _lib.load().moe_add_rmsnorm_fp8, x.data_ptr(), ptr(h),
+          weight.data_ptr(), scale.numel(), n, eps, added, q.data_ptr(), scale.data_ptr(), ptr(norm))
     return (total, q, scale, norm) if return_norm else (total, q, scale)
 
 
@@ -496,48 +508,64 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
     [N, K], fp32 up to the one rounding. Operands are both bf16 (K a multiple of 8) or both
     float8_e4m3fn with fp32 row scales ``x_scale`` [...] and ``w_scale`` [N] (K a multiple of
     16). ``bias`` [N] is bf16 or fp32, ``mul`` and ``residual`` [..., N] bf16; ``activation`` is
-    None, "relu", "silu", "gelu" or "gelu_tanh". Rows of ``w`` (and of a 2-D ``x``) may be
-    strided, as in a slice of a packed weight, if each starts at a multiple of 16 bytes."""
-    _need_cuda(x, w)
-    if activation not in _lib.ACTIVATIONS:
+    None, "relu", "silu", "gelu" or "gelu_tanh". Rows of ``w`` may be strided, as in a slice of a
+    packed weight, if each starts at a multiple of 16 bytes; rows of ``x`` that are not so are
+    copied."""
+    if not (x.is_cuda and w.is_cuda):
+        _need_cuda(x, w)
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {list(_lib.ACTIVATIONS)} (got {activation!r})")
-    if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, FP8):
-        raise ValueError(f"x and w must both be bfloat16 or float8_e4m3fn (got {x.dtype}, {w.dtype})")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not match")
-    _same_device(x, w=w, x_scale=x_scale, w_scale=w_scale, bias=bias, mul=mul, residual=residual)
+    kind = x.dtype
+    if w.dtype is not kind or not (kind is torch.bfloat16 or kind is FP8):
+        raise ValueError(f"x and w must both be bfloat16 or float8_e4m3fn (got {kind}, {w.dtype})")
+    shape, dev = x.shape, x.get_device()
+    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1]:
+        raise ValueError(f"x {tuple(shape)} and w {tuple(w.shape)} do not match")
+    if w.get_device() != dev:
+        raise ValueError(f"w is on {w.device}, x on {x.device}")
     n, k = w.shape
-    size = x.element_size()
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    rows = x2.shape[0]
-    if x2.stride(1) != 1 or x2.stride(0) < k or x2.stride(0) * size % 16 or x2.data_ptr() % 16:
-        x2 = _aligned(x2)
-    if w.stride(1) != 1 or w.stride(0) < k or w.stride(0) * size % 16 or w.data_ptr() % 16:
+    size = 1 if kind is FP8 else 2
+    if not (len(shape) == 2 and _rows_in_place(x, k, size)):
+        x = _input(x, kind, "x").view(-1, k)
+    rows, ldx = x.shape[0], x.stride(0)
+    if rows < 2:
+        ldx = k
+    if not _rows_in_place(w, k, size):
         raise ValueError("rows of w must be contiguous and start at multiples of 16 bytes")
-    dtype = _lib.WEIGHTS_BF16
-    if x.dtype == FP8:
-        dtype = _lib.WEIGHTS_FP8_E4M3
-        x_scale, w_scale = _scales(x_scale, "x_scale", rows), _scales(w_scale, "w_scale", n)
+    if kind is FP8:
+        x_scale = _vector(x_scale, _F32, "x_scale", rows, dev).data_ptr()
+        w_scale = _vector(w_scale, _F32, "w_scale", n, dev).data_ptr()
     elif x_scale is not None or w_scale is not None:
         raise ValueError("bf16 operands take no scales")
+    out_shape = (*shape[:-1], n)
+    bias_f32 = 0
     if bias is not None:
-        if bias.dtype not in (torch.bfloat16, torch.float32) or bias.numel() != n:
-            raise ValueError(f"bias must be {n} bfloat16 or float32 values")
-        bias = bias.contiguous()
-    shape = (*x.shape[:-1], n)
-    for name, t in (("mul", mul), ("residual", residual)):
-        if t is not None and t.shape != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, the output {shape}")
+        bias = _vector(bias, _BIAS, "bias", n, dev)
+        bias_f32 = int(bias.dtype is torch.float32)
     if mul is not None:
-        mul = _aligned(_bf16(mul, "mul"))
+        if mul.shape != out_shape:
+            raise ValueError(f"mul has shape {tuple(mul.shape)}, the output {out_shape}")
+        mul = _input(mul, torch.bfloat16, "mul", dev)
     if residual is not None:
-        residual = _aligned(_bf16(residual, "residual"))
-    out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
-    _call("linear", x.device, _lib.load().moe_linear, x2.data_ptr(), x2.stride(0), ptr(x_scale),
-          w.data_ptr(), w.stride(0), ptr(w_scale), dtype, rows, k, n, ptr(bias),
-          int(bias is not None and bias.dtype == torch.float32), _lib.ACTIVATIONS[activation],
-          ptr(mul), ptr(residual), out.data_ptr())
+        if residual.shape != out_shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, the output {out_shape}")
+        residual = _input(residual, torch.bfloat16, "residual", dev)
+    out = torch.empty(out_shape, dtype=torch.bfloat16, device=x.device)
+    _call("linear", dev, _lib.load().moe_linear, x.data_ptr(), ldx, x_scale, w.data_ptr(),
+          w.stride(0) if n > 1 else k, w_scale,
+          _lib.WEIGHTS_FP8_E4M3 if size == 1 else _lib.WEIGHTS_BF16, rows, k, n, ptr(bias), bias_f32,
+          act, ptr(mul), ptr(residual), out.data_ptr())
     return out
+
+
+def _rows_in_place(t: torch.Tensor, k: int, size: int) -> bool:
+    """Whether the rows of ``t`` [rows, k] can be read where they are: contiguous, at multiples of
+    16 bytes and at most 4 MiB apart."""
+    ld, step = t.stride()
+    if t.shape[0] < 2:
+        ld = k
+    return (step == 1 or k == 1) and k <= ld <= (1 << 22) // size and not (ld * size | t.data_ptr()) & 15
 
 
 def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
@@ -549,37 +577,42 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
     with one power-of-two scale per 32 columns; pair outputs are rounded to bf16 and their weighted
     sum, fp32 with bf16 weights, once more. ``top_k_index`` [T, k] int64 holds experts in
     [0, E)."""
-    _need_cuda(q, scale, top_k_index, top_k_weights, gate_up, down)
-    _same_device(q, scale=scale, top_k_index=top_k_index, top_k_weights=top_k_weights,
-                 gate_up=gate_up, down=down, gate_up_scale=gate_up_scale, down_scale=down_scale)
-    if q.dtype != FP8 or q.dim() != 2:
-        raise ValueError(f"q must be float8_e4m3fn [T, H] (got {q.dtype}, {tuple(q.shape)})")
-    if gate_up.dtype != FP8 or down.dtype != FP8:
-        raise ValueError("experts_fp8 takes float8_e4m3fn experts (see fp8.quantize_experts)")
-    gu, gus, _ = expert_weight(gate_up, gate_up_scale, "gate_up")
-    dn, dns, _ = expert_weight(down, down_scale, "down")
-    _check_row_major(gu, dn)
+    if not (q.is_cuda and gate_up.is_cuda and down.is_cuda and top_k_index.is_cuda):
+        _need_cuda(q, gate_up, down, top_k_index)
+    if q.dim() != 2:
+        raise ValueError(f"q must be float8_e4m3fn [T, H] (got {tuple(q.shape)})")
+    q = _input(q, FP8, "q")
     tokens, hidden = q.shape
-    if gu.dim() != 3 or gu.shape[2] != hidden or gu.shape[1] % 2:
-        raise ValueError(f"gate_up shape {tuple(gu.shape)} does not fit rows of {hidden}")
-    nexp, inter = gu.shape[0], gu.shape[1] // 2
-    if dn.shape != (nexp, hidden, inter):
-        raise ValueError(f"down shape {tuple(dn.shape)} != {(nexp, hidden, inter)}")
-    if top_k_index.dtype != torch.long or top_k_index.dim() != 2 or top_k_index.shape[0] != tokens:
+    dev = q.get_device()
+    if gate_up.dtype is not FP8 or down.dtype is not FP8:
+        raise ValueError("experts_fp8 takes float8_e4m3fn experts (see fp8.quantize_experts)")
+    _check_row_major(gate_up, down)
+    if gate_up.dim() != 3 or gate_up.shape[2] != hidden or gate_up.shape[1] % 2:
+        raise ValueError(f"gate_up shape {tuple(gate_up.shape)} does not fit rows of {hidden}")
+    nexp, two_i, _ = gate_up.shape
+    inter = two_i // 2
+    if down.shape != (nexp, hidden, inter):
+        raise ValueError(f"down shape {tuple(down.shape)} != {(nexp, hidden, inter)}")
+    if top_k_index.dtype is not torch.long or top_k_index.dim() != 2 or top_k_index.shape[0] != tokens:
         raise ValueError(f"top_k_index must be int64 [{tokens}, k]")
     if top_k_weights.shape != top_k_index.shape:
         raise ValueError(f"top_k_weights must be {tuple(top_k_index.shape)}")
+    for name, t in (("gate_up", gate_up), ("down", down), ("top_k_index", top_k_index),
+                    ("top_k_weights", top_k_weights)):
+        if t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
     top_k = top_k_index.shape[1]
-    scale = _scales(scale, "scale", tokens)
-    q = _aligned(q)
-    idx = top_k_index.contiguous()
+    scale = _vector(scale, _F32, "scale", tokens, dev)
+    gus = _vector(gate_up_scale, _F32, "gate_up_scale", nexp * two_i, dev)
+    dns = _vector(down_scale, _F32, "down_scale", nexp * hidden, dev)
+    idx = top_k_index if top_k_index.is_contiguous() else top_k_index.contiguous()
     wts = top_k_weights.to(torch.bfloat16).contiguous()
     out = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=q.device)
     lib = _lib.load()
     nbytes = lib.moe_experts_fp8_workspace_bytes(tokens, hidden, nexp, top_k, inter)
     # a workspace of the call's own: one captured in a graph belongs to that graph
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
-    _call("experts_fp8", q.device, lib.moe_experts_fp8_forward, q.data_ptr(), scale.data_ptr(), tokens,
-          hidden, nexp, top_k, inter, idx.data_ptr(), wts.data_ptr(), gu.data_ptr(), gus.data_ptr(),
-          dn.data_ptr(), dns.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
+    _call("experts_fp8", dev, lib.moe_experts_fp8_forward, q.data_ptr(), scale.data_ptr(), tokens,
+          hidden, nexp, top_k, inter, idx.data_ptr(), wts.data_ptr(), gate_up.data_ptr(),
+          gus.data_ptr(), down.data_ptr(), dns.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
