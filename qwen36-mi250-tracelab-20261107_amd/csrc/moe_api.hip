@@ -969,7 +969,7 @@ bool apart(const Span* in, int ni, const Span* out, int no) {
 
 struct Experts8Ws {
   int *counts, *offsets, *order, *table, *scratch;
-  uint8_t *aq, *asc;
+  uint8_t *aq, *asc, *yexp;
   uint16_t* y;
   size_t bytes;
   int MT, bm;
@@ -979,15 +979,18 @@ Experts8Ws carve_experts8(void* base, int T, int H, int E, int k, int I) {
   Experts8Ws w{};
   const int P = T * k;
   w.bm = rows_tile_rows(T, k, E);
-  w.MT = max_tiles_of(T, k, E, w.bm, 0);
-  w.counts = c.take<int>(E);
-  w.offsets = c.take<int>(E);
-  w.order = c.take<int>(P);
-  w.table = c.take<int>(3 * (size_t)w.MT + 1);
-  w.scratch = c.take<int>(sort_scratch_bytes(P, E) / sizeof(int) + 1);
   w.aq = c.take<uint8_t>((size_t)P * I);
   w.asc = c.take<uint8_t>((size_t)((I + 127) / 128) * P * 4);
-  w.y = c.take<uint16_t>((size_t)P * H);
+  if (w.bm) {
+    w.MT = max_tiles_of(T, k, E, w.bm, 0);
+    w.counts = c.take<int>(E);
+    w.offsets = c.take<int>(E);
+    w.order = c.take<int>(P);
+    w.table = c.take<int>(3 * (size_t)w.MT + 1);
+    w.scratch = c.take<int>(sort_scratch_bytes(P, E) / sizeof(int) + 1);
+    w.y = c.take<uint16_t>((size_t)P * H);
+    w.yexp = c.take<uint8_t>((size_t)P * (H / 32));
+  }
   w.bytes = c.off;
   return w;
 }
@@ -1229,26 +1232,35 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
   CHECK_ARG(workspace && workspace_bytes >= w.bytes, "experts_fp8: workspace too small: %zu < %zu",
             workspace_bytes, w.bytes);
   hipStream_t s = (hipStream_t)stream;
-  HIP_TRY(launch_route_sort(nullptr, 0, nullptr, top_k_index, T, E, k, w.bm, 0, nullptr, nullptr,
-                            nullptr, w.counts, w.offsets, w.order, w.table, w.MT, w.scratch, s),
-          "sort launch");
+  const uint16_t* wts = static_cast<const uint16_t*>(top_k_weights);
   RowsGemm a{};
   a.x = static_cast<const uint8_t*>(q), a.ldx = H, a.xbytes = (long long)T * H;
   a.w = static_cast<const uint8_t*>(gate_up), a.ldw = H, a.estride = 2LL * I * H;
   a.xs = x_scale, a.ws = gu_scale;
   a.N = I, a.Kb = H;
-  a.table = w.table, a.order = w.order, a.MT = w.MT, a.topk = k;
+  a.topk = k;
   a.P = (long long)T * k;
   a.aq = w.aq, a.asc = w.asc;
+  if (w.bm) {
+    HIP_TRY(launch_route_sort(nullptr, 0, nullptr, top_k_index, T, E, k, w.bm, 0, nullptr, nullptr,
+                              nullptr, w.counts, w.offsets, w.order, w.table, w.MT, w.scratch, s),
+            "sort launch");
+    a.table = w.table, a.order = w.order, a.MT = w.MT;
+  } else {
+    a.ids = top_k_index;
+  }
   HIP_TRY(launch_rows_gemm(kRowsGateUp, 1, a, w.bm, s), "gate_up launch");
   a.x = w.aq, a.ldx = I;
   a.w = static_cast<const uint8_t*>(down), a.ldw = I, a.estride = (long long)H * I;
   a.xs = nullptr, a.ws = dn_scale;
   a.N = H, a.Kb = I;
-  a.out = w.y;
+  if (!w.bm) {
+    a.out = static_cast<uint16_t*>(out), a.wts = wts;
+    return hip_check(launch_rows_pairs_down(a, T, s), "down launch");
+  }
+  a.out = w.y, a.yexp = w.yexp;
   HIP_TRY(launch_rows_gemm(kRowsDown, 1, a, w.bm, s), "down launch");
-  return hip_check(launch_combine(w.y, static_cast<const uint16_t*>(top_k_weights), k, nullptr,
-                                  nullptr, 0, nullptr, static_cast<uint16_t*>(out), T, H, 0, s),
+  return hip_check(launch_rows_combine(w.y, w.yexp, wts, T, H, k, static_cast<uint16_t*>(out), s),
                    "combine launch");
 }
 

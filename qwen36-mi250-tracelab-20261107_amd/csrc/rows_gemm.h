@@ -47,7 +47,7 @@ struct RowsGemm {
   const void* bias;
   const uint16_t* mul;
   const uint16_t* res;
-  uint16_t* out;      // also kRowsDown's y
+  uint16_t* out;      // also kRowsDown's y [P, N] fp16
   int act, bias_f32;
   // experts: the sorted pairs and their tiles (route_sort.hip)
   const int* table;
@@ -56,6 +56,10 @@ struct RowsGemm {
   long long P;        // pairs
   uint8_t* aq;        // [P, I] e4m3, in sorted order
   uint8_t* asc;       // [ceil(I / 128)][P][4]: biased exponent of each group of 32
+  uint8_t* yexp;      // [P, N / 32]: exponent + 128 of 32 values of y
+  // a few pairs (kRowsGateUp without a table, launch_rows_pairs_down): pair p is its own sorted row
+  const long long* ids;
+  const uint16_t* wts;
 };
 
 typedef int v8i_t __attribute__((ext_vector_type(8)));
@@ -111,58 +115,69 @@ __device__ __forceinline__ void rows_act(float (&v)[C], int act) {
   }
 }
 
-// kRowsLinear: C neighbouring outputs of token row m from n on (as far as N goes), whose sums are
-// v. Where N is a multiple of C they are one aligned access.
-template <int C>
-__device__ __forceinline__ void rows_linear_out(const RowsGemm& a, long long m, int n, float xs,
-                                                const float (&ws)[C], const float (&bias)[C],
-                                                float (&v)[C]) {
-  static_assert(C == 4 || C == 8, "8 or 16 bytes");
-  const long long at = m * a.N + n;
-  const bool vec = a.N % C == 0;
-  auto load = [&](const uint16_t* p, uint16_t (&d)[C]) __attribute__((always_inline)) {
-    if (vec) {
-      __builtin_memcpy(d, __builtin_assume_aligned(p + at, 2 * C), 2 * C);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) d[i] = n + i < a.N ? p[at + i] : 0;
-    }
-  };
-  uint16_t mv[C], rv[C];
-  if (a.mul) load(a.mul, mv);
-  if (a.res) load(a.res, rv);
+// kRowsLinear: eight neighbouring outputs of a token row, whose sums are v, from their mul and
+// residual (bf16), as bf16.
+struct RowsOperands {
+  uint4 mul, res;
+};
+__device__ __forceinline__ uint4 rows_linear_value(const RowsGemm& a, float xs, const float (&ws)[8],
+                                                   const float (&bias)[8], const RowsOperands& op,
+                                                   float (&v)[8]) {
   if (a.ws) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] *= xs * ws[i];
+    for (int i = 0; i < 8; ++i) v[i] *= xs * ws[i];
   }
 #pragma unroll
-  for (int i = 0; i < C; ++i) v[i] += bias[i];
+  for (int i = 0; i < 8; ++i) v[i] += bias[i];
   rows_act(v, a.act);
   if (a.mul) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] *= bf_bits2f(mv[i]);
+    for (int i = 0; i < 8; ++i) v[i] *= i & 1 ? bf_hi((&op.mul.x)[i / 2]) : bf_lo((&op.mul.x)[i / 2]);
   }
   if (a.res) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] += bf_bits2f(rv[i]);
+    for (int i = 0; i < 8; ++i) v[i] += i & 1 ? bf_hi((&op.res.x)[i / 2]) : bf_lo((&op.res.x)[i / 2]);
   }
-  uint32_t o[C / 2];
+  return make_uint4(pack_bf2_rne(v[0], v[1]), pack_bf2_rne(v[2], v[3]), pack_bf2_rne(v[4], v[5]),
+                    pack_bf2_rne(v[6], v[7]));
+}
+// Eight neighbouring bf16 at any element: one 16-byte access (gfx950 takes it at any address).
+__device__ __forceinline__ uint4 rows_load8(const uint16_t* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// The operands and the outputs of the last columns of a row of N not a multiple of 8: `in` of eight.
+__device__ __forceinline__ uint4 rows_load_tail(const uint16_t* p, int in) {
+  uint32_t d[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int i = 0; i < C; i += 2) o[i / 2] = pack_bf2_rne(v[i], v[i + 1]);
-  if (vec) {
-    __builtin_memcpy(__builtin_assume_aligned(a.out + at, 2 * C), o, 2 * C);
+  for (int i = 0; i < 7; ++i)
+    if (i < in) d[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+  return make_uint4(d[0], d[1], d[2], d[3]);
+}
+__device__ __forceinline__ void rows_linear_load(const RowsGemm& a, long long m, int n,
+                                                 RowsOperands& o) {
+  const long long at = m * a.N + n;
+  const int in = a.N - n;
+  if (a.mul) o.mul = in >= 8 ? rows_load8(a.mul + at) : rows_load_tail(a.mul + at, in);
+  if (a.res) o.res = in >= 8 ? rows_load8(a.res + at) : rows_load_tail(a.res + at, in);
+}
+__device__ __forceinline__ void rows_linear_store(const RowsGemm& a, long long m, int n, uint4 v) {
+  uint16_t* out = a.out + m * a.N + n;
+  if (n + 8 <= a.N) {
+    __builtin_memcpy(out, &v, 16);
   } else {
+    const uint32_t o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (n + i < a.N) a.out[at + i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
+    for (int i = 0; i < 7; ++i)
+      if (n + i < a.N) out[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
   }
 }
 // Their weight scales and biases (zeros past N).
-template <int C>
-__device__ __forceinline__ void rows_linear_cols(const RowsGemm& a, int n, float (&ws)[C],
-                                                 float (&bias)[C]) {
+__device__ __forceinline__ void rows_linear_cols(const RowsGemm& a, int n, float (&ws)[8],
+                                                 float (&bias)[8]) {
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const bool in = n + i < a.N;
     ws[i] = a.ws && in ? a.ws[n + i] : 0.f;
     bias[i] = !a.bias || !in ? 0.f
@@ -215,19 +230,43 @@ __device__ __forceinline__ void rows_gate_up_cols(const RowsGemm& a, int e, int 
   for (int i = 0; i < 8; ++i) sg[i] = s[i], su[i] = s[a.N + i];
 }
 
-// kRowsDown: outputs n .. n + 7 of pair row p, whose scales are ws.
-__device__ __forceinline__ void rows_down_out(const RowsGemm& a, long long p, int n,
-                                              const float (&ws)[8], const float (&v)[8]) {
+// kRowsDown: outputs n .. n + 7 of pair row p, whose scales are ws, on their way to the weighted sum:
+// fp16 values of a power of two 2^ex per 32 columns, ex + 128 in a byte of its own, the largest
+// between 2^14 and 2^15. At bf16's size, its error (2^-12 of a value) does not show in the sum,
+// where bf16's (2^-9) was as large as the result's own rounding. The four lanes of 32 columns are
+// neighbours and all called; live: the row is stored.
+__device__ __forceinline__ void rows_down_out(const RowsGemm& a, bool live, long long p, int n,
+                                              const float (&ws)[8], float (&v)[8]) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] *= ws[i];
+    amax = fmaxf(amax, finite_abs(v[i]));
+  }
+  amax = fmaxf(amax, dppf<kDppXor1>(amax));
+  amax = fmaxf(amax, dppf<kDppXor2>(amax));
+  const int ex = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120);
+  const float m = __uint_as_float((uint32_t)(127 - ex) << 23);
+  if (!live || n >= a.N) return;
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) o[i / 2] = pack_bf2_rne(v[i] * ws[i], v[i + 1] * ws[i + 1]);
+  for (int i = 0; i < 8; i += 2)
+    o[i / 2] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)(v[i] * m), (_Float16)(v[i + 1] * m)});
   st16(a.out + p * a.N + n, make_uint4(o[0], o[1], o[2], o[3]));
+  a.yexp[p * (a.N / 32) + n / 32] = (uint8_t)(ex + 128);
 }
 
 // es: bytes of an element. max_tiles: entries of the tile table at most (experts), built with
 // rows_tile_rows rows a tile. hipErrorInvalidValue for shapes outside the contract above.
+// rows_tile_rows 0: so few pairs that each is a tile of its own (ids in place of a table).
 int rows_tile_rows(int T, int k, int E);
 hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_rows,
                             hipStream_t s);
+// kRowsDown and the weighted sum for tile_rows 0: out [T, N] = bf16(sum_j wts_tj ws acc).
+hipError_t launch_rows_pairs_down(const RowsGemm& a, int T, hipStream_t s);
+// out [T, H] = bf16(sum_j w_tj y_tj) for y as kRowsDown writes it.
+hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w, int T, int H,
+                               int k, uint16_t* out, hipStream_t s);
 
 }  // namespace moe

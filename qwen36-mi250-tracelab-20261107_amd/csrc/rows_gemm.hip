@@ -21,6 +21,12 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
     t.r1 = min(t.r0 + tile_rows, (long long)a.M);
     return t.r0 < a.M;
   }
+  if (MODE == kRowsGateUp && a.ids) {
+    t.e = (int)a.ids[tile];
+    t.r0 = tile;
+    t.r1 = tile + 1;
+    return true;
+  }
   if (tile >= a.table[3 * a.MT]) return false;
   t.e = a.table[tile];
   t.r0 = a.table[a.MT + tile];
@@ -29,9 +35,10 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
 }
 
 // Few token rows: 16 NB weight rows times 16 MB token rows a workgroup, K split over its W
-// waves, operands straight from memory into the matrix instructions; the waves' sums meet in
-// LDS in a fixed order. Bound by the stream of weights.
-template <int ES, int MODE, int NB, int MB, int W>
+// waves, operands straight from memory into the matrix instructions, the loads of U steps (16 KiB
+// of weights a wave) together; the waves' sums meet in LDS in a fixed order. Bound by the stream of
+// weights, for one token by its latency.
+template <int ES, int MODE, int NB, int MB, int W, int U>
 __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   __shared__ f32x4_t red[W][NB * MB][64];
   RowsTile t;
@@ -50,12 +57,40 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
       n = min((int)(blockIdx.x * NB + b) * 16 + lr, a.N - 1);
     wp[b] = a.w + t.e * a.estride + n * a.ldw;
   }
+  auto token = [&](long long r) __attribute__((always_inline)) {
+    return MODE != kRowsGateUp ? r : (a.ids ? r : (long long)a.order[r]) / a.topk;
+  };
   long long row[MB];
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     const long long r = min(t.r0 + m * 16 + lr, t.r1 - 1);
-    row[m] = MODE == kRowsGateUp ? a.order[r] / a.topk : r;
-    xp[m] = a.x + row[m] * a.ldx;
+    row[m] = r;
+    xp[m] = a.x + token(r) * a.ldx;
+  }
+  // The epilogue's thread: eight neighbouring outputs of a token row. What it needs beside the sums
+  // is requested here, so that it does not wait for memory at the end.
+  constexpr int PER = MODE == kRowsGateUp ? 4 : 2 * NB;  // threads of a row
+  static_assert(16 * MB * PER <= W * 64, "a thread each");
+  const int tid = threadIdx.x, erow = tid / PER, ec = tid - erow * PER;
+  const long long er = t.r0 + erow, err = min(er, t.r1 - 1);
+  const int en = (MODE == kRowsGateUp ? blockIdx.x * 32 : blockIdx.x * NB * 16) + ec * 8;
+  const bool mine = erow < 16 * MB && (MODE != kRowsLinear || (er < t.r1 && en < a.N));
+  float ews[8], eother[8], exs = 1.f;
+  RowsOperands eop;
+  long long pair = 0;
+  if (mine) {
+    if constexpr (MODE == kRowsGateUp) {
+      rows_gate_up_cols(a, t.e, en, ews, eother);
+      exs = a.xs[token(err)];
+    } else if constexpr (MODE == kRowsLinear) {
+      rows_linear_cols(a, en, ews, eother);
+      rows_linear_load(a, er, en, eop);
+      if (a.xs) exs = a.xs[er];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ews[j] = a.ws[(long long)t.e * a.N + min(en, a.N - 8) + j];
+      pair = a.order[err];
+    }
   }
   f32x4_t acc[NB][MB];
 #pragma unroll
@@ -64,30 +99,43 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
     for (int m = 0; m < MB; ++m) acc[b][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const int nch = (a.Kb + 127) / 128;
   const int c0 = (int)((long long)nch * wave / W), c1 = (int)((long long)nch * (wave + 1) / W);
-  for (int c = c0; c < c1; ++c) {
-    // past the row's end: its last 16 bytes again, the token's as zeros
-    const int k0 = c * 128 + kq * 16, k1 = k0 + 64;
-    const int o0 = min(k0, a.Kb - 16), o1 = min(k1, a.Kb - 16);
-    uint4 xv[MB][2];
+  for (int c = c0; c < c1; c += U) {
+    uint4 wv[U][NB][2], xv[U][MB][2];
+    int sv[U][MB];
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-      xv[m][0] = ld16(xp[m] + o0);
-      xv[m][1] = ld16(xp[m] + o1);
-      if (k0 >= a.Kb) xv[m][0] = make_uint4(0u, 0u, 0u, 0u);
-      if (k1 >= a.Kb) xv[m][1] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int s = 0; s < U; ++s) {
+      // past the wave's part or the row's end: bytes there again, the token's as zeros
+      const int k0 = (c + s) * 128 + kq * 16, k1 = k0 + 64;
+      const int o0 = min(k0, a.Kb - 16), o1 = min(k1, a.Kb - 16);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const uint4 w0 = ld16_stream(wp[b] + o0), w1 = ld16_stream(wp[b] + o1);
+      for (int b = 0; b < NB; ++b) {
+        wv[s][b][0] = ld16_stream(wp[b] + o0);
+        wv[s][b][1] = ld16_stream(wp[b] + o1);
+      }
 #pragma unroll
       for (int m = 0; m < MB; ++m) {
-        if (MODE == kRowsDown) {
-          const int sb = a.asc[(c * a.P + row[m]) * 4 + kq];
-          acc[b][m] = rows_mma_scaled(w0, w1, xv[m][0], xv[m][1], sb, acc[b][m]);
-        } else {
-          acc[b][m] = rows_mma<ES>(w0, w1, xv[m][0], xv[m][1], acc[b][m]);
-        }
+        xv[s][m][0] = ld16(xp[m] + o0);
+        xv[s][m][1] = ld16(xp[m] + o1);
+        if (MODE == kRowsDown) sv[s][m] = a.asc[(min(c + s, nch - 1) * a.P + row[m]) * 4 + kq];
       }
+    }
+#pragma unroll
+    for (int s = 0; s < U; ++s) {
+      const int k0 = (c + s) * 128 + kq * 16, k1 = k0 + 64;
+      const int end = c + s < c1 ? a.Kb : 0;
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        if (k0 >= end) xv[s][m][0] = make_uint4(0u, 0u, 0u, 0u);
+        if (k1 >= end) xv[s][m][1] = make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+          acc[b][m] = MODE == kRowsDown
+                          ? rows_mma_scaled(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1],
+                                            sv[s][m], acc[b][m])
+                          : rows_mma<ES>(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1], acc[b][m]);
     }
   }
 #pragma unroll
@@ -95,49 +143,30 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) red[wave][m * NB + b][lane] = acc[b][m];
   __syncthreads();
-  // Eight neighbouring outputs a thread: quads (b, 2 h) and (b, 2 h + 1) of token row (m, lr) lie 16
-  // lanes apart.
-  const int tid = threadIdx.x;
-  constexpr int PER = MODE == kRowsGateUp ? 4 : 2 * NB;  // threads of a row
-  for (int i = tid; i < 16 * MB * PER; i += W * 64) {
-    const int row = i / PER, c = i - row * PER, m = row >> 4;
-    auto sum = [&](int b, float (&v)[8]) __attribute__((always_inline)) {
-      const int l = (row & 15) + (c & 1) * 32;
-      f32x4_t s0 = red[0][m * NB + b][l], s1 = red[0][m * NB + b][l + 16];
+  if (!mine) return;  // (whole waves, or for kRowsLinear threads that share nothing)
+  // quads (b, 2 h) and (b, 2 h + 1) of token row (m, lr) lie 16 lanes apart
+  auto sum = [&](int b, float (&v)[8]) __attribute__((always_inline)) {
+    const int l = (erow & 15) + (ec & 1) * 32, at = (erow >> 4) * NB + b;
+    f32x4_t s0 = red[0][at][l], s1 = red[0][at][l + 16];
 #pragma unroll
-      for (int w = 1; w < W; ++w) s0 += red[w][m * NB + b][l], s1 += red[w][m * NB + b][l + 16];
+    for (int w = 1; w < W; ++w) s0 += red[w][at][l], s1 += red[w][at][l + 16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = s0[j], v[4 + j] = s1[j];
-    };
-    const long long r = t.r0 + row;
-    const bool live = r < t.r1;
-    const long long rr = min(r, t.r1 - 1);
-    float v[8];
-    sum(c >> 1, v);
-    if constexpr (MODE == kRowsGateUp) {
-      const int n = blockIdx.x * 32 + c * 8;
-      float u[8], sg[8], su[8];
-      sum(2 + (c >> 1), u);
-      rows_gate_up_cols(a, t.e, n, sg, su);
-      rows_gate_up_out(a, live, r, n, sg, su, a.xs[a.order[rr] / a.topk], v, u);
-      // the scales behind the last group
-      const int grp = blockIdx.x + 1 + c;
-      if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + c < 4 && live)
-        a.asc[((grp >> 2) * a.P + r) * 4 + (grp & 3)] = 127;
-    } else {
-      const int n = blockIdx.x * NB * 16 + c * 8;
-      if (!live || n >= a.N) continue;
-      float ws[8];
-      if (MODE == kRowsLinear) {
-        float bias[8];
-        rows_linear_cols(a, n, ws, bias);
-        rows_linear_out(a, r, n, a.xs ? a.xs[r] : 1.f, ws, bias, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ws[j] = a.ws[(long long)t.e * a.N + n + j];
-        rows_down_out(a, a.order[r], n, ws, v);
-      }
-    }
+    for (int j = 0; j < 4; ++j) v[j] = s0[j], v[4 + j] = s1[j];
+  };
+  float v[8];
+  sum(ec >> 1, v);
+  if constexpr (MODE == kRowsGateUp) {
+    float u[8];
+    sum(2 + (ec >> 1), u);
+    rows_gate_up_out(a, er < t.r1, er, en, ews, eother, exs, v, u);
+    // the scales behind the last group
+    const int grp = blockIdx.x + 1 + ec;
+    if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + ec < 4 && er < t.r1)
+      a.asc[((grp >> 2) * a.P + er) * 4 + (grp & 3)] = 127;
+  } else if constexpr (MODE == kRowsLinear) {
+    rows_linear_store(a, er, en, rows_linear_value(a, exs, ews, eother, eop, v));
+  } else {
+    rows_down_out(a, er < t.r1, pair, en, ews, v);
   }
 }
 
@@ -187,7 +216,14 @@ __device__ __forceinline__ void tile_mma(const Frag& w, const Frag& t, uint32_t 
   }
 }
 // The last product's passes, before anything else reads the sums.
-__device__ __forceinline__ void mma_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+template <int NA, int NB>
+__device__ __forceinline__ void mma_done(f32x4_t (&acc)[NA][NB]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < NA; ++x)
+#pragma unroll
+    for (int y = 0; y < NB; ++y) asm volatile("" : "+a"(acc[x][y]));
+}
 template <int OFF>
 __device__ __forceinline__ uint32_t lds_read4(uint32_t addr) {
   uint32_t r;
@@ -301,8 +337,8 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
     // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows
-    const uint32_t r = MODE == kRowsGateUp ? (uint32_t)(((i / (NA / 4)) & 1) * a.N +
-                                                        (i / (NA / 2)) * 8 * NA + (i % (NA / 4)) * 32)
+    constexpr int Q = MODE == kRowsGateUp ? NA / 4 : 1;
+    const uint32_t r = MODE == kRowsGateUp ? (uint32_t)((i / Q & 1) * a.N + i / (2 * Q) * 8 * NA + i % Q * 32)
                                            : 32u * i;
     wrow[i] = __builtin_amdgcn_readfirstlane((int)r < wrows ? r * ldw : 0);
   }
@@ -473,7 +509,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
   }
   wait_loads(0);
-  mma_done();
+  mma_done(acc);
 
   // ---- epilogue: half of the wave's token blocks at a time through LDS, row by row, so that one small
   // loop serves all of the sums (unrolled over the registers it was 80 KB of instructions, which took
@@ -482,6 +518,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   static_assert(4 * HB * 16 * kStride * 4 <= S::kLds, "the waves' parts");
   constexpr int PER = (MODE == kRowsGateUp ? NA : 2 * NA);  // lanes of a row, eight outputs each
   constexpr int RPI = 64 / PER;
+  static_assert(PER >= 4 && 64 % PER == 0 && 16 % (64 / PER) == 0, "whole turns in a token block");
   float* part = reinterpret_cast<float*>(lds) + wave * HB * 16 * kStride;
   const int c = lane % PER, rsub = lane / PER;
   const int n = n0 + wm * (S::kOut / 2) + c * 8;
@@ -493,11 +530,82 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   else
 #pragma unroll
     for (int i = 0; i < 8; ++i) ws[i] = a.ws[(long long)t.e * a.N + min(n + i, a.N - 1)];
-  __syncthreads();  // the stages have been read
+  // A token block (UE rows of a lane) at a time. What the next one needs beside the sums is
+  // requested first, without branches, behind which the compiler would wait for everything in flight,
+  // the stores too: lanes and operands that are not there read 16 bytes of a weight row.
+  constexpr int UE = 16 / RPI;
+  struct Rows {
+    long long r[UE];  // row to store, -1: none
+    float xs[UE];
+    RowsOperands op[UE];
+  };
+  const bool eight = n + 8 <= a.N;  // else some of the last columns, or none
+  const uint16_t* idle = reinterpret_cast<const uint16_t*>(a.w);
+  auto fetch = [&](int b, Rows& o) __attribute__((always_inline)) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int blocks = min(HB, nb - half * HB);
-    if (blocks <= 0) break;
+    for (int i = 0; i < UE; ++i) {
+      const int row = (2 * b + wn) * 16 + rsub + i * RPI;
+      const bool live = row < ntok;
+      o.r[i] = live ? t.r0 + row : -1;
+      o.xs[i] = 1.f;
+      if constexpr (MODE == kRowsLinear) {
+        const long long at = (t.r0 + row) * a.N + n;
+        o.op[i].mul = rows_load8(a.mul && live && eight ? a.mul + at : idle);
+        o.op[i].res = rows_load8(a.res && live && eight ? a.res + at : idle);
+        o.xs[i] = *(a.xs && live ? a.xs + t.r0 + row : reinterpret_cast<const float*>(a.w));
+      } else {
+        const int pair = a.order[min(t.r0 + row, t.r1 - 1)];
+        if (MODE == kRowsGateUp)
+          o.xs[i] = a.xs[pair / a.topk];
+        else
+          o.r[i] = live ? pair : -1;
+      }
+    }
+  };
+  // (LDS is read by asm: before reads of its own the compiler would wait for the DMA loads, as which
+  // it counts the stores here too)
+  auto finish = [&](int b, const Rows& o) __attribute__((always_inline)) {
+    const int blk = b < HB ? b : b - HB;
+    const uint32_t src = lds_addr(part) + ((blk * 16 + rsub) * kStride + c * 8) * 4;
+    u32x4v raw[UE][MODE == kRowsGateUp ? 4 : 2];
+    static_for<UE>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, off = i * RPI * kStride * 4;
+      raw[i][0] = lds_read_frag<off>(src);
+      raw[i][1] = lds_read_frag<off + 16>(src);
+      if constexpr (MODE == kRowsGateUp) {
+        raw[i][2] = lds_read_frag<off + 32 * NA>(src);
+        raw[i][3] = lds_read_frag<off + 32 * NA + 16>(src);
+      }
+    });
+    lds_frags_ready();
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+#pragma unroll
+      for (u32x4v& f : raw[i]) after_wait(f);
+    }
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+      float v[8], u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = __uint_as_float(raw[i][j / 4][j % 4]);
+        if constexpr (MODE == kRowsGateUp) u[j] = __uint_as_float(raw[i][2 + j / 4][j % 4]);
+      }
+      if constexpr (MODE == kRowsGateUp) {
+        rows_gate_up_out(a, o.r[i] >= 0, o.r[i], n, ws, other, o.xs[i], v, u);
+      } else if constexpr (MODE == kRowsLinear) {
+        RowsOperands op = o.op[i];
+        const bool some = o.r[i] >= 0 && n < a.N;
+        if (some && !eight) rows_linear_load(a, o.r[i], n, op);
+        const uint4 w = rows_linear_value(a, o.xs[i], ws, other, op, v);
+        if (some) rows_linear_store(a, o.r[i], n, w);
+      } else {
+        rows_down_out(a, o.r[i] >= 0, o.r[i], n, ws, v);
+      }
+    }
+  };
+  auto stage = [&](auto hc) __attribute__((always_inline)) {
+    constexpr int half = decltype(hc)::value;
 #pragma unroll
     for (int i = 0; i < HB; ++i)
 #pragma unroll
@@ -508,41 +616,135 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
       }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses run in order)
-    for (int row = rsub; row < blocks * 16; row += RPI) {
-      const long long r = t.r0 + (2 * (half * HB + (row >> 4)) + wn) * 16 + (row & 15);
-      const float* src = part + row * kStride + c * 8;
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = src[j];
-      const bool live = r < t.r1;
-      if constexpr (MODE == kRowsGateUp) {
-        float u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = src[8 * NA + j];
-        const float xs = a.xs[a.order[min(r, t.r1 - 1)] / a.topk];
-        rows_gate_up_out(a, live, r, n, ws, other, xs, v, u);
-      } else if (live && n < a.N) {
-        if constexpr (MODE == kRowsLinear)
-          rows_linear_out(a, r, n, a.xs ? a.xs[r] : 1.f, ws, other, v);
-        else
-          rows_down_out(a, a.order[r], n, ws, v);
-      }
-    }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
+  };
+  Rows cur, next;
+  fetch(0, cur);
+  __syncthreads();  // the stages have been read
+#pragma unroll 1
+  for (int b = 0; b < nb; ++b) {
+    if (b == 0) stage(c0);
+    if (b == HB) stage(c1);
+    fetch(min(b + 1, nb - 1), next);
+    finish(b, cur);
+    cur = next;  // (where the compiler waits for it)
   }
 }
 
-template <int ES, int MODE, int MB>
+// The down product of a few pairs and their weighted sum: 16 outputs of one token a workgroup, a wave
+// a pair.
+constexpr int kPairWaves = 8;
+__global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a) {
+  __shared__ float part[kPairWaves][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, kq = lane >> 4;
+  const int n0 = blockIdx.x * 16;  // N is a multiple of 32
+  const int nch = (a.Kb + 127) / 128;
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = wave; j < a.topk; j += kPairWaves) {
+    const long long p = (long long)blockIdx.y * a.topk + j;
+    const long long e = a.ids[p];
+    const uint8_t* wp = a.w + e * a.estride + (n0 + lr) * a.ldw;
+    const uint8_t* xp = a.x + p * a.ldx;  // every column of the product is the pair's row
+    const float w = bf_bits2f(a.wts[p]);
+    const float* sd = a.ws + e * a.N + n0 + 4 * kq;
+    float sw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sw[i] = sd[i];
+    f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 4;
+    for (int c = 0; c < nch; c += U) {
+      uint4 wv[U][2], xv[U][2];
+      int sv[U];
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        const int k0 = (c + s) * 128 + kq * 16;
+        const int o0 = min(k0, a.Kb - 16), o1 = min(k0 + 64, a.Kb - 16);
+        wv[s][0] = ld16_stream(wp + o0), wv[s][1] = ld16_stream(wp + o1);
+        xv[s][0] = ld16(xp + o0), xv[s][1] = ld16(xp + o1);
+        sv[s] = a.asc[(min(c + s, nch - 1) * a.P + p) * 4 + kq];
+      }
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        const int k0 = (c + s) * 128 + kq * 16;
+        if (k0 >= a.Kb) xv[s][0] = make_uint4(0u, 0u, 0u, 0u);
+        if (k0 + 64 >= a.Kb) xv[s][1] = make_uint4(0u, 0u, 0u, 0u);
+        acc = rows_mma_scaled(wv[s][0], wv[s][1], xv[s][0], xv[s][1], sv[s], acc);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total[i] = fmaf(w, acc[i] * sw[i], total[i]);
+  }
+  if (lr == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][4 * kq + i] = total[i];
+  }
+  __syncthreads();
+  const int n = threadIdx.x;
+  if (n >= 16) return;
+  float s = part[0][n];
+#pragma unroll
+  for (int w = 1; w < kPairWaves; ++w) s += part[w][n];
+  a.out[(long long)blockIdx.y * a.N + n0 + n] = f2bf_bits(s);
+}
+
+// Eight outputs a thread, the pairs' values of eight pairs requested together. Bound by memory.
+__global__ __launch_bounds__(256) void k_rows_combine(const uint16_t* y, const uint8_t* yexp,
+                                                      const uint16_t* w, int T, int H, int k,
+                                                      uint16_t* out) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int per = H / 8;
+  const long long t = i / per;
+  if (t >= T) return;
+  const int c = (int)(i - t * per) * 8;
+  float acc[8] = {};
+  for (int j0 = 0; j0 < k; j0 += 8) {
+    uint4 v[8];
+    float m[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long long p = t * k + min(j0 + j, k - 1);
+      v[j] = ld16_stream(y + p * H + c);
+      m[j] = bf_bits2f(w[p]) * __uint_as_float((uint32_t)(yexp[p * (H / 32) + c / 32] - 1) << 23);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= k) break;
+      const uint32_t u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, u[x]);
+        acc[2 * x] = fmaf((float)h[0], m[j], acc[2 * x]);
+        acc[2 * x + 1] = fmaf((float)h[1], m[j], acc[2 * x + 1]);
+      }
+    }
+  }
+  st16(out + t * H + c, make_uint4(pack_bf2_rne(acc[0], acc[1]), pack_bf2_rne(acc[2], acc[3]),
+                                   pack_bf2_rne(acc[4], acc[5]), pack_bf2_rne(acc[6], acc[7])));
+}
+
+template <int ES, int MODE, int NB, int MB, int W, int U>
 hipError_t launch_few(const RowsGemm& a, hipStream_t s) {
-  constexpr int NB = MODE == kRowsGateUp ? 4 : 2, W = 4;
   const long long cols = MODE == kRowsGateUp ? a.N / 32 : (a.N + 16 * NB - 1) / (16 * NB);
-  const long long tiles = MODE == kRowsLinear ? (a.M + 16 * MB - 1) / (16 * MB) : a.MT;
+  const long long tiles = MODE == kRowsLinear     ? (a.M + 16 * MB - 1) / (16 * MB)
+                          : a.ids && !a.table ? a.P
+                                              : a.MT;
   if (tiles <= 0 || cols <= 0) return hipSuccess;
   if (tiles > 65535 || cols > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W>), dim3((unsigned)cols, (unsigned)tiles),
+  hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W, U>), dim3((unsigned)cols, (unsigned)tiles),
                      dim3(W * 64), 0, s, a);
   return hipGetLastError();
+}
+template <int ES>
+hipError_t launch_few_linear(const RowsGemm& a, int mb, hipStream_t s) {
+  const char* e = getenv("ROWS_NB");
+  const int nb = e ? atoi(e) : a.N <= 4096 ? 1 : 2;
+  if (mb == 4) return launch_few<ES, kRowsLinear, 2, 4, 4, 2>(a, s);
+  if (mb == 2) return launch_few<ES, kRowsLinear, 2, 2, 8, 2>(a, s);
+  if (nb == 1) return launch_few<ES, kRowsLinear, 1, 1, 8, 4>(a, s);
+  if (nb == 3) return launch_few<ES, kRowsLinear, 1, 1, 8, 2>(a, s);
+  return launch_few<ES, kRowsLinear, 2, 1, 8, 2>(a, s);
 }
 
 // A kernel's dynamic LDS above the default limit, allowed once per device.
@@ -583,9 +785,9 @@ hipError_t launch_tile(const RowsGemm& a, hipStream_t s) {
 bool tile_fits(RowsMode mode, const RowsGemm& a) {
   const long long most = 1LL << 31;
   if (256 * a.ldw >= most || 256 * a.ldx >= most) return false;
+  if (mode == kRowsLinear) return 512LL * a.N < most;
   if (mode == kRowsGateUp) return 2LL * a.N * a.ldw < most && a.xbytes < most;
-  if (mode == kRowsDown) return (a.Kb + 127) / 128 * a.P * 4 < most;
-  return true;
+  return (a.Kb + 127) / 128 * a.P * 4 < most;
 }
 
 template <int ES>
@@ -593,7 +795,7 @@ hipError_t launch_linear(const RowsGemm& a, int c, hipStream_t s) {
   if (c == 256) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
   if (c == 128) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
   if (c == 64) return launch_tile<ES, kRowsLinear, 2, 2>(a, s);
-  return c ? launch_few<ES, kRowsLinear, 4>(a, s) : launch_few<ES, kRowsLinear, 1>(a, s);
+  return launch_few_linear<ES>(a, c ? c : 1, s);
 }
 
 }  // namespace
@@ -602,7 +804,23 @@ int rows_tile_rows(int T, int k, int E) {
   const long long P = (long long)T * k;
   const char* e = getenv("ROWS_TILE");
   if (e) return atoi(e);
-  return P > 32LL * E ? 192 : P > 16LL * E ? 64 : 16;
+  return P <= 16 ? 0 : P > 12LL * E ? 192 : 16;
+}
+
+hipError_t launch_rows_pairs_down(const RowsGemm& a, int T, hipStream_t s) {
+  if (T <= 0) return hipSuccess;
+  if (T > 65535 || a.N % 32 || a.Kb < 16 || a.Kb % 16) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k_rows_pairs_down, dim3(a.N / 16, T), dim3(kPairWaves * 64), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w, int T, int H,
+                               int k, uint16_t* out, hipStream_t s) {
+  if (T <= 0) return hipSuccess;
+  const long long grid = ((long long)T * (H / 8) + 255) / 256;
+  if (H % 32 || grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)grid), dim3(256), 0, s, y, yexp, w, T, H, k, out);
+  return hipGetLastError();
 }
 
 hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_rows,
@@ -610,21 +828,25 @@ hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_r
   if (a.Kb < 16 || a.Kb % 16 || a.N < 1) return hipErrorInvalidValue;
   if (mode == kRowsLinear) {
     const char* e = getenv("ROWS_LIN");
-    int c = e ? atoi(e) : a.M <= 16 ? 0 : a.M <= 64 ? 1 : 256;
+    int c = e ? atoi(e) : a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 64 ? 4 : 256;
     if (!e && c == 256) {
       auto n = [&](long long b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
       c = n(256) >= 200 ? 256 : n(128) >= 128 ? 128 : 64;
     }
-    if (!tile_fits(mode, a) && c > 1) c = 1;
+    if (!tile_fits(mode, a) && c > 4) c = 4;
     return es == 2 ? launch_linear<2>(a, c, s) : launch_linear<1>(a, c, s);
   }
   if (es != 1 || a.N % 32) return hipErrorInvalidValue;
   if (mode == kRowsGateUp) {
     if (tile_rows == 192) return tile_fits(mode, a) ? launch_tile<1, kRowsGateUp, 8, 6>(a, s) : hipErrorInvalidValue;
-    return tile_rows == 16 ? launch_few<1, kRowsGateUp, 1>(a, s) : launch_few<1, kRowsGateUp, 4>(a, s);
+    return tile_rows <= 16   ? launch_few<1, kRowsGateUp, 4, 1, 4, 1>(a, s)
+           : tile_rows == 32 ? launch_few<1, kRowsGateUp, 4, 2, 8, 2>(a, s)
+                             : launch_few<1, kRowsGateUp, 4, 4, 4, 2>(a, s);
   }
   if (tile_rows == 192) return tile_fits(mode, a) ? launch_tile<1, kRowsDown, 8, 6>(a, s) : hipErrorInvalidValue;
-  return tile_rows == 16 ? launch_few<1, kRowsDown, 1>(a, s) : launch_few<1, kRowsDown, 4>(a, s);
+  return tile_rows == 16   ? launch_few<1, kRowsDown, 2, 1, 4, 1>(a, s)
+         : tile_rows == 32 ? launch_few<1, kRowsDown, 4, 2, 4, 2>(a, s)
+                           : launch_few<1, kRowsDown, 2, 4, 4, 2>(a, s);
 }
 
 }  // namespace moe
