@@ -120,6 +120,7 @@ __device__ __forceinline__ void rows_act(float (&v)[C], int act) {
 struct RowsOperands {
   uint4 mul, res;
 };
+template <bool WITH = true>  // whether there can be mul or residual
 __device__ __forceinline__ uint4 rows_linear_value(const RowsGemm& a, float xs, const float (&ws)[8],
                                                    const float (&bias)[8], const RowsOperands& op,
                                                    float (&v)[8]) {
@@ -130,11 +131,11 @@ __device__ __forceinline__ uint4 rows_linear_value(const RowsGemm& a, float xs, 
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += bias[i];
   rows_act(v, a.act);
-  if (a.mul) {
+  if (WITH && a.mul) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= i & 1 ? bf_hi((&op.mul.x)[i / 2]) : bf_lo((&op.mul.x)[i / 2]);
   }
-  if (a.res) {
+  if (WITH && a.res) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += i & 1 ? bf_hi((&op.res.x)[i / 2]) : bf_lo((&op.res.x)[i / 2]);
   }
@@ -162,10 +163,17 @@ __device__ __forceinline__ void rows_linear_load(const RowsGemm& a, long long m,
   if (a.mul) o.mul = in >= 8 ? rows_load8(a.mul + at) : rows_load_tail(a.mul + at, in);
   if (a.res) o.res = in >= 8 ? rows_load8(a.res + at) : rows_load_tail(a.res + at, in);
 }
+// NT: past the caches, for outputs much larger than they are.
+template <bool NT>
 __device__ __forceinline__ void rows_linear_store(const RowsGemm& a, long long m, int n, uint4 v) {
+  typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
   uint16_t* out = a.out + m * a.N + n;
   if (n + 8 <= a.N) {
-    __builtin_memcpy(out, &v, 16);
+    const u32x4_any w = {v.x, v.y, v.z, v.w};
+    if (NT)
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(out));
+    else
+      *reinterpret_cast<u32x4_any*>(out) = w;
   } else {
     const uint32_t o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll

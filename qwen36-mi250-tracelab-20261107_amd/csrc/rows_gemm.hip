@@ -164,7 +164,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
     if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + ec < 4 && er < t.r1)
       a.asc[((grp >> 2) * a.P + er) * 4 + (grp & 3)] = 127;
   } else if constexpr (MODE == kRowsLinear) {
-    rows_linear_store(a, er, en, rows_linear_value(a, exs, ews, eother, eop, v));
+    rows_linear_store<false>(a, er, en, rows_linear_value(a, exs, ews, eother, eop, v));
   } else {
     rows_down_out(a, er < t.r1, pair, en, ews, v);
   }
@@ -488,6 +488,15 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     ra[0] = ra[1], ra[1] = ra[2], ra[2] = t0;
     rb[0] = rb[1], rb[1] = u0;
   };
+  // A row's scale or pair, for the epilogue
+  uint32_t meta = 0;
+  if (tid < ntok) {
+    if (MODE == kRowsLinear)
+      meta = a.xs ? __float_as_uint(a.xs[t.r0 + tid]) : 0;
+    else
+      meta = a.order[t.r0 + tid];
+    if (MODE == kRowsGateUp) meta = __float_as_uint(a.xs[meta / a.topk]);
+  }
   // (in the order in which the steps issue them: tokens, then weights one further on)
   static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(0, ra[0]), k); });
   static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(0, rb[0]), k); });
@@ -515,11 +524,14 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   // loop serves all of the sums (unrolled over the registers it was 80 KB of instructions, which took
   // longer to fetch than a tile of K = 1024 to multiply) and a row's outputs are stored together
   constexpr int kStride = 16 * NA + 4;  // floats of a row: 16 bytes on, so that eight rows differ in banks
-  static_assert(4 * HB * 16 * kStride * 4 <= S::kLds, "the waves' parts");
+  constexpr int kPart = HB * 16 * kStride;
+  static_assert(4 * kPart * 4 + S::kTRows * 4 <= S::kLds, "the waves' parts and the rows' values");
   constexpr int PER = (MODE == kRowsGateUp ? NA : 2 * NA);  // lanes of a row, eight outputs each
   constexpr int RPI = 64 / PER;
   static_assert(PER >= 4 && 64 % PER == 0 && 16 % (64 / PER) == 0, "whole turns in a token block");
-  float* part = reinterpret_cast<float*>(lds) + wave * HB * 16 * kStride;
+  constexpr int UE = 16 / RPI;  // rows of a lane in a token block
+  float* part = reinterpret_cast<float*>(lds) + wave * kPart;
+  uint32_t* metas = reinterpret_cast<uint32_t*>(lds) + 4 * kPart;
   const int c = lane % PER, rsub = lane / PER;
   const int n = n0 + wm * (S::kOut / 2) + c * 8;
   float ws[8], other[8];  // scales, and the up scales or the bias
@@ -530,80 +542,6 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   else
 #pragma unroll
     for (int i = 0; i < 8; ++i) ws[i] = a.ws[(long long)t.e * a.N + min(n + i, a.N - 1)];
-  // A token block (UE rows of a lane) at a time. What the next one needs beside the sums is
-  // requested first, without branches, behind which the compiler would wait for everything in flight,
-  // the stores too: lanes and operands that are not there read 16 bytes of a weight row.
-  constexpr int UE = 16 / RPI;
-  struct Rows {
-    long long r[UE];  // row to store, -1: none
-    float xs[UE];
-    RowsOperands op[UE];
-  };
-  const bool eight = n + 8 <= a.N;  // else some of the last columns, or none
-  const uint16_t* idle = reinterpret_cast<const uint16_t*>(a.w);
-  auto fetch = [&](int b, Rows& o) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < UE; ++i) {
-      const int row = (2 * b + wn) * 16 + rsub + i * RPI;
-      const bool live = row < ntok;
-      o.r[i] = live ? t.r0 + row : -1;
-      o.xs[i] = 1.f;
-      if constexpr (MODE == kRowsLinear) {
-        const long long at = (t.r0 + row) * a.N + n;
-        o.op[i].mul = rows_load8(a.mul && live && eight ? a.mul + at : idle);
-        o.op[i].res = rows_load8(a.res && live && eight ? a.res + at : idle);
-        o.xs[i] = *(a.xs && live ? a.xs + t.r0 + row : reinterpret_cast<const float*>(a.w));
-      } else {
-        const int pair = a.order[min(t.r0 + row, t.r1 - 1)];
-        if (MODE == kRowsGateUp)
-          o.xs[i] = a.xs[pair / a.topk];
-        else
-          o.r[i] = live ? pair : -1;
-      }
-    }
-  };
-  // (LDS is read by asm: before reads of its own the compiler would wait for the DMA loads, as which
-  // it counts the stores here too)
-  auto finish = [&](int b, const Rows& o) __attribute__((always_inline)) {
-    const int blk = b < HB ? b : b - HB;
-    const uint32_t src = lds_addr(part) + ((blk * 16 + rsub) * kStride + c * 8) * 4;
-    u32x4v raw[UE][MODE == kRowsGateUp ? 4 : 2];
-    static_for<UE>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value, off = i * RPI * kStride * 4;
-      raw[i][0] = lds_read_frag<off>(src);
-      raw[i][1] = lds_read_frag<off + 16>(src);
-      if constexpr (MODE == kRowsGateUp) {
-        raw[i][2] = lds_read_frag<off + 32 * NA>(src);
-        raw[i][3] = lds_read_frag<off + 32 * NA + 16>(src);
-      }
-    });
-    lds_frags_ready();
-#pragma unroll
-    for (int i = 0; i < UE; ++i) {
-#pragma unroll
-      for (u32x4v& f : raw[i]) after_wait(f);
-    }
-#pragma unroll
-    for (int i = 0; i < UE; ++i) {
-      float v[8], u[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = __uint_as_float(raw[i][j / 4][j % 4]);
-        if constexpr (MODE == kRowsGateUp) u[j] = __uint_as_float(raw[i][2 + j / 4][j % 4]);
-      }
-      if constexpr (MODE == kRowsGateUp) {
-        rows_gate_up_out(a, o.r[i] >= 0, o.r[i], n, ws, other, o.xs[i], v, u);
-      } else if constexpr (MODE == kRowsLinear) {
-        RowsOperands op = o.op[i];
-        const bool some = o.r[i] >= 0 && n < a.N;
-        if (some && !eight) rows_linear_load(a, o.r[i], n, op);
-        const uint4 w = rows_linear_value(a, o.xs[i], ws, other, op, v);
-        if (some) rows_linear_store(a, o.r[i], n, w);
-      } else {
-        rows_down_out(a, o.r[i] >= 0, o.r[i], n, ws, v);
-      }
-    }
-  };
   auto stage = [&](auto hc) __attribute__((always_inline)) {
     constexpr int half = decltype(hc)::value;
 #pragma unroll
@@ -617,16 +555,103 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses run in order)
   };
-  Rows cur, next;
-  fetch(0, cur);
-  __syncthreads();  // the stages have been read
-#pragma unroll 1
-  for (int b = 0; b < nb; ++b) {
-    if (b == 0) stage(c0);
+  // mul and residual of a token block. They are requested two blocks ahead and before the stores of the
+  // block then at hand, because loads and stores complete in order: a load behind the stores would wait
+  // for them, and with it everything. For the same reason there is no branch here (behind one the
+  // compiler waits for all in flight): what is not there reads 16 bytes of a weight row.
+  struct Ops {
+    RowsOperands row[UE];
+  };
+  const bool eight = n + 8 <= a.N;  // else some of the last columns, or none
+  const uint16_t* idle = reinterpret_cast<const uint16_t*>(a.w);
+  auto row_of = [&](int b, int i) __attribute__((always_inline)) {  // in the tile
+    return (2 * b + wn) * 16 + rsub + i * RPI;
+  };
+  auto fetch = [&](int b, Ops& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+      const int row = row_of(b, i);
+      const bool there = row < ntok && eight;
+      const long long at = (t.r0 + row) * a.N + n;
+      o.row[i].mul = rows_load8(a.mul && there ? a.mul + at : idle);
+      o.row[i].res = rows_load8(a.res && there ? a.res + at : idle);
+    }
+  };
+  // Token block b. LDS is read by asm: before reads of its own the compiler would wait for the DMA
+  // loads, as which it counts the stores here too.
+  auto finish = [&](auto with, int b, Ops& o) __attribute__((always_inline)) {
+    constexpr bool WITH = decltype(with)::value;
     if (b == HB) stage(c1);
-    fetch(min(b + 1, nb - 1), next);
-    finish(b, cur);
-    cur = next;  // (where the compiler waits for it)
+    const uint32_t src = lds_addr(part) + (((b < HB ? b : b - HB) * 16 + rsub) * kStride + c * 8) * 4;
+    const uint32_t msrc = lds_addr(metas) + row_of(b, 0) * 4;
+    u32x4v raw[UE][MODE == kRowsGateUp ? 4 : 2];
+    uint32_t mv[UE];
+    static_for<UE>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, off = i * RPI * kStride * 4;
+      raw[i][0] = lds_read_frag<off>(src);
+      raw[i][1] = lds_read_frag<off + 16>(src);
+      if constexpr (MODE == kRowsGateUp) {
+        raw[i][2] = lds_read_frag<off + 32 * NA>(src);
+        raw[i][3] = lds_read_frag<off + 32 * NA + 16>(src);
+      }
+      mv[i] = lds_read4<i * RPI * 4>(msrc);
+    });
+    lds_frags_ready();
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+      asm volatile("" : "+v"(mv[i]));
+#pragma unroll
+      for (u32x4v& f : raw[i]) after_wait(f);
+    }
+    uint4 w[UE];
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+      const bool live = row_of(b, i) < ntok;
+      const long long r = t.r0 + row_of(b, i);
+      float v[8], u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = __uint_as_float(raw[i][j / 4][j % 4]);
+        if constexpr (MODE == kRowsGateUp) u[j] = __uint_as_float(raw[i][2 + j / 4][j % 4]);
+      }
+      if constexpr (MODE == kRowsGateUp) {
+        rows_gate_up_out(a, live, r, n, ws, other, __uint_as_float(mv[i]), v, u);
+      } else if constexpr (MODE == kRowsDown) {
+        rows_down_out(a, live, mv[i], n, ws, v);
+      } else {
+        RowsOperands op;
+        if (WITH) {
+          op = o.row[i];
+          if (live && n < a.N && !eight) rows_linear_load(a, r, n, op);
+        }
+        w[i] = rows_linear_value<WITH>(a, __uint_as_float(mv[i]), ws, other, op, v);
+      }
+    }
+    if constexpr (MODE == kRowsLinear) {
+      if (WITH) fetch(min(b + 2, nb - 1), o);
+#pragma unroll
+      for (int i = 0; i < UE; ++i)
+        if (row_of(b, i) < ntok && n < a.N)
+          rows_linear_store<NA == 8>(a, t.r0 + row_of(b, i), n, w[i]);
+    }
+  };
+  __syncthreads();  // the stages have been read
+  if (tid < S::kTRows) metas[tid] = meta;
+  stage(c0);
+  __syncthreads();
+  if (nb <= 0) return;
+  Ops s0, s1;
+  if (MODE == kRowsLinear && (a.mul || a.res)) {
+    fetch(0, s0);
+    fetch(min(1, nb - 1), s1);
+#pragma unroll 1
+    for (int b = 0; b < nb; b += 2) {
+      finish(std::true_type{}, b, s0);
+      finish(std::true_type{}, b + 1, s1);  // (of no live rows if nb is odd)
+    }
+  } else {
+#pragma unroll 1
+    for (int b = 0; b < nb; ++b) finish(std::false_type{}, b, s0);
   }
 }
 
