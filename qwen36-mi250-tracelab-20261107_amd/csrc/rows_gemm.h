@@ -115,18 +115,18 @@ __device__ __forceinline__ void rows_act(float (&v)[C], int act) {
   }
 }
 
-// kRowsLinear: eight neighbouring outputs of a token row, whose sums are v, from their mul and
-// residual (bf16), as bf16.
+// kRowsLinear: eight neighbouring outputs of a token row, whose sums times the row's scale are v,
+// from their mul and residual (bf16), as bf16.
 struct RowsOperands {
   uint4 mul, res;
 };
 template <bool WITH = true>  // whether there can be mul or residual
-__device__ __forceinline__ uint4 rows_linear_value(const RowsGemm& a, float xs, const float (&ws)[8],
+__device__ __forceinline__ uint4 rows_linear_value(const RowsGemm& a, const float (&ws)[8],
                                                    const float (&bias)[8], const RowsOperands& op,
                                                    float (&v)[8]) {
   if (a.ws) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= xs * ws[i];
+    for (int i = 0; i < 8; ++i) v[i] *= ws[i];
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += bias[i];
@@ -200,18 +200,18 @@ __device__ __forceinline__ int group_exponent(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   return max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
 }
-// kRowsGateUp: columns n .. n + 7 of sorted row r, whose sums are g and u and whose scales sg and su
-// (the token's included); the four lanes of a group of 32 are neighbours. Every lane of the wave
+// kRowsGateUp: columns n .. n + 7 of sorted row r, whose sums times the token's scale are g and u and
+// whose scales are sg and su; the four lanes of a group of 32 are neighbours. Every lane of the wave
 // calls; live: the row is stored. Scales of the groups that fill up the last 128 columns are
 // written as 1 (their values are read as zeros).
 __device__ __forceinline__ void rows_gate_up_out(const RowsGemm& a, bool live, long long r, int n,
-                                                 const float (&sg)[8], const float (&su)[8], float xs,
+                                                 const float (&sg)[8], const float (&su)[8],
                                                  const float (&g)[8], const float (&u)[8]) {
   float v[8], amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float gv = g[i] * (xs * sg[i]);
-    v[i] = rows_gate(gv, gv) * (u[i] * (xs * su[i]));
+    const float gv = g[i] * sg[i];
+    v[i] = rows_gate(gv, gv) * (u[i] * su[i]);
     amax = fmaxf(amax, finite_abs(v[i]));
   }
   amax = fmaxf(amax, dppf<kDppXor1>(amax));

@@ -1,4 +1,6 @@
 // Kernels of rows_gemm.h.
+#include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -158,13 +160,19 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   if constexpr (MODE == kRowsGateUp) {
     float u[8];
     sum(2 + (ec >> 1), u);
-    rows_gate_up_out(a, er < t.r1, er, en, ews, eother, exs, v, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= exs, u[j] *= exs;
+    rows_gate_up_out(a, er < t.r1, er, en, ews, eother, v, u);
     // the scales behind the last group
     const int grp = blockIdx.x + 1 + ec;
     if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + ec < 4 && er < t.r1)
       a.asc[((grp >> 2) * a.P + er) * 4 + (grp & 3)] = 127;
   } else if constexpr (MODE == kRowsLinear) {
-    rows_linear_store<false>(a, er, en, rows_linear_value(a, exs, ews, eother, eop, v));
+    if (a.xs) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= exs;
+    }
+    rows_linear_store<false>(a, er, en, rows_linear_value(a, ews, eother, eop, v));
   } else {
     rows_down_out(a, er < t.r1, pair, en, ews, v);
   }
@@ -187,11 +195,18 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 //
 // A step's products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0). Between
 // its matrix instructions, which leave three of four issue slots free, each reads from LDS, early, the
-// half that the next one needs, and the last two issue the DMA loads; they read the next step's
-// first halves, the tokens' into the registers that held half 1. One barrier a step, after the second
-// quarter: the step has been read by all, and the next one has arrived. (With the loads issued
-// together after the barrier and the reads after each block's products, a step of 256 x 256
-// took 4400 cycles; its products take 2048.)
+// half that the next one needs; the last two read the next step's first halves, the tokens' into the
+// registers that held half 1. Two barriers a step. After the first quarter the step's tokens have been
+// read by all: their stage is loaded during the second. After the third, its weights have: theirs is
+// loaded during the fourth. Behind the first the next step's weights have arrived, behind the second
+// its tokens: either has a step and a half. (With one barrier, after the second quarter, the tokens
+// had one step, less than L2 takes where there are 192 rows. With the loads issued together after it
+// and the reads after each block's products, a step of 256 x 256 took 4400 cycles; its products
+// take 2048.)
+//
+// A workgroup walks over tiles, as many workgroups as the chip holds. The next tile's first two steps
+// are requested before the present one's epilogue, which needs only the third weight stage of LDS, so
+// that memory is not idle meanwhile.
 struct Frag {
   u32x4v v[2];
 };
@@ -214,6 +229,24 @@ __device__ __forceinline__ void tile_mma(const Frag& w, const Frag& t, uint32_t 
       asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(acc) : "v"(w8), "v"(t8));
     }
   }
+}
+__device__ __forceinline__ void tie(uint4& v) {
+  asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+}
+// (also as asm: the compiler would read all sums of a tile ahead of the loop that stores them, into
+// registers that are not there)
+__device__ __forceinline__ void lds_write_scaled_sums(uint32_t addr, const f32x4_t& acc, float s) {
+  f32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(f) : "a"(acc[i]));
+    v[i] = f * s;
+  }
+  asm volatile("ds_write_b128 %0, %1" : : "v"(addr), "v"(v) : "memory");
+}
+__device__ __forceinline__ void lds_write_sums(uint32_t addr, const f32x4_t& acc) {
+  asm volatile("ds_write_b128 %0, %1" : : "v"(addr), "a"(acc) : "memory");
 }
 // The last product's passes, before anything else reads the sums.
 template <int NA, int NB>
@@ -250,7 +283,8 @@ struct TileShape {
   static constexpr bool kScaled = MODE == kRowsDown;
   static constexpr int kAStage = kWRows * 128;
   static constexpr int kBStage = kTRows * 128 + (kScaled ? kTRows * 4 : 0);
-  static constexpr int kLds = kSA * kAStage + kSB * kBStage;
+  static constexpr int kMetas = kSA * kAStage + kSB * kBStage;  // kRowsDown: the rows' pairs
+  static constexpr int kLds = kMetas + (kScaled ? kTRows * 4 : 0);
   static constexpr int kOut = MODE == kRowsGateUp ? kWRows / 2 : kWRows;  // outputs per workgroup
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
@@ -262,16 +296,25 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   constexpr int HA = NA / 2, HB = NB / 2;
   constexpr int LA = S::kWRows / 32, LB = S::kTRows / 32;  // loads of a wave and step
   extern __shared__ uint4 smem[];
-  // Workgroup id % 8 is its XCD. Experts: the ncol workgroups of one tile on one XCD, so they share its
-  // token rows in that L2. Linear: each XCD walks its own part of the output in columns of four tiles
-  // of token rows, whose workgroups share both operands.
-  int tile, col;
-  {
-    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  const int lr = lane & 15, kq = lane >> 4;
+  char* lds = reinterpret_cast<char*>(smem);
+
+  struct Tile {
+    int e, r0, ntok, n0;  // expert, first token row (or sorted pair), rows, first output
+  };
+  // Tile `id`, id % 8 being this workgroup's XCD. Experts: the ncol tiles of the same rows on one XCD,
+  // so they share them in that L2. Linear: each XCD walks its own part of the output in columns of
+  // four tiles of token rows, whose workgroups share both operands.
+  auto tile_of = [&](int id, Tile& t) __attribute__((always_inline)) {
+    int tile, col;
+    const int xcd = id & 7, j = id >> 3;
     if (MODE == kRowsLinear) {
       const int all = ncol * ntile, per = (all + 7) / 8;
       const int pos = xcd * per + j;
-      if (j >= per || pos >= all) return;
+      if (j >= per || pos >= all) return false;
       const int g = pos / (4 * ncol), in = pos - g * 4 * ncol;
       const int high = min(4, ntile - 4 * g);
       col = in / high;
@@ -280,26 +323,20 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
       tile = (j / ncol) * 8 + xcd;
       col = j - (j / ncol) * ncol;
     }
-  }
-  RowsTile t;
-  if (!rows_tile<MODE>(a, tile, S::kTRows, t)) return;
-  const int ntok = (int)(t.r1 - t.r0);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
-  const int lr = lane & 15, kq = lane >> 4;
-  char* lds = reinterpret_cast<char*>(smem);
+    RowsTile r;
+    if (!rows_tile<MODE>(a, tile, S::kTRows, r)) return false;
+    t.e = r.e, t.r0 = (int)r.r0, t.ntok = (int)(r.r1 - r.r0), t.n0 = col * S::kOut;
+    return true;
+  };
+  int id = blockIdx.x;
+  Tile cur, next;
+  if (!tile_of(id, cur)) return;
 
   // ---- DMA: the wave's load i fills LDS rows (wave + 4 i) 8 .. + 7, lane l unit l & 7 of row l >> 3
   constexpr uint32_t kNowhere = 0x80000000u;  // past the end of any of the buffers
   constexpr int SPAN = MODE == kRowsGateUp ? 2 * NA : 4 * NA;
   const int grow = lane >> 3, row0 = wave * 8 + grow;
-  const int n0 = col * S::kOut;
   const uint32_t ldw = (uint32_t)a.ldw, ldx = (uint32_t)a.ldx;
-  const int wrows = MODE == kRowsGateUp ? 2 * a.N - n0 : min(S::kWRows, a.N - n0);
-  const __amdgpu_buffer_rsrc_t wbuf = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(a.w + t.e * a.estride + (long long)n0 * a.ldw), 0,
-      (uint32_t)(wrows - 1) * ldw + a.Kb, 0x00020000);
   uint32_t wunit[2], woff[2];  // by load parity (the key of row0 + 32)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -307,44 +344,52 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     wunit[i] = ((lane & 7) ^ key) * 16;
     woff[i] = row0 * ldw + wunit[i];
   }
-  const uint8_t* xbase = MODE == kRowsGateUp ? a.x : a.x + t.r0 * a.ldx;
-  const uint32_t xbytes = MODE == kRowsGateUp ? (uint32_t)a.xbytes : (uint32_t)(ntok - 1) * ldx + a.Kb;
-  const __amdgpu_buffer_rsrc_t xbuf =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(xbase), 0, xbytes, 0x00020000);
   const uint32_t tunit = ((lane & 7) ^ grow) * 16;
-  uint32_t toff[MODE == kRowsGateUp ? LB : 1];
-  if (MODE == kRowsGateUp) {
-#pragma unroll
-    for (int i = 0; i < LB; ++i) {
-      const int r = row0 + 32 * i;
-      toff[i] = r < ntok ? (uint32_t)(a.order[t.r0 + r] / a.topk) * ldx + tunit : kNowhere;
-    }
-  } else {
-    toff[0] = row0 * ldx + tunit;
-  }
-  const __amdgpu_buffer_rsrc_t sbuf = __builtin_amdgcn_make_buffer_rsrc(
-      SC ? a.asc + t.r0 * 4 : nullptr, 0,
-      SC ? (uint32_t)(((a.Kb + 127) / 128 - 1) * a.P * 4 + ntok * 4) : 0, 0x00020000);
   // (the last wave's scale load, past the stage's rows, repeats the one before)
   const int srow = min(wave, S::kTRows / 64 - 1) * 64;
-  const uint32_t soff = srow + lane < ntok ? (srow + lane) * 4 : kNowhere;
   const int nd = (a.Kb + 127) / 128;
+  // Where a tile's loads come from. A load's uniform offset never passes its buffer's end: the rows of a
+  // group past the last row are those of the first group again.
+  __amdgpu_buffer_rsrc_t wbuf, xbuf, sbuf;
+  uint32_t wrow[LA], xrow[LB], toff[MODE == kRowsGateUp ? LB : 1], soff;
+  auto set_sources = [&](const Tile& t) __attribute__((always_inline)) {
+    const int wrows = MODE == kRowsGateUp ? 2 * a.N - t.n0 : min(S::kWRows, a.N - t.n0);
+    wbuf = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(a.w + t.e * a.estride + (long long)t.n0 * a.ldw), 0,
+        (uint32_t)(wrows - 1) * ldw + a.Kb, 0x00020000);
+    const uint8_t* xbase = MODE == kRowsGateUp ? a.x : a.x + t.r0 * a.ldx;
+    const uint32_t xbytes =
+        MODE == kRowsGateUp ? (uint32_t)a.xbytes : (uint32_t)(t.ntok - 1) * ldx + a.Kb;
+    xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(xbase), 0, xbytes, 0x00020000);
+    sbuf = __builtin_amdgcn_make_buffer_rsrc(
+        SC ? a.asc + (long long)t.r0 * 4 : nullptr, 0,
+        SC ? (uint32_t)((nd - 1) * a.P * 4 + t.ntok * 4) : 0, 0x00020000);
+    soff = srow + lane < t.ntok ? (srow + lane) * 4 : kNowhere;
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+      // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows
+      constexpr int Q = MODE == kRowsGateUp ? NA / 4 : 1;
+      const uint32_t r = MODE == kRowsGateUp
+                             ? (uint32_t)((i / Q & 1) * a.N + i / (2 * Q) * 8 * NA + i % Q * 32)
+                             : 32u * i;
+      wrow[i] = __builtin_amdgcn_readfirstlane((int)r < wrows ? r * ldw : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      xrow[i] =
+          __builtin_amdgcn_readfirstlane(MODE != kRowsGateUp && 32 * i < t.ntok ? 32u * i * ldx : 0);
+    if constexpr (MODE == kRowsGateUp) {
+#pragma unroll
+      for (int i = 0; i < LB; ++i) {
+        const int tok = a.order[t.r0 + min(row0 + 32 * i, t.ntok - 1)] / a.topk;
+        toff[i] = row0 + 32 * i < t.ntok ? (uint32_t)tok * ldx + tunit : kNowhere;
+      }
+    } else {
+      toff[0] = row0 * ldx + tunit;
+    }
+  };
   // The loads of step d; past the last one, of nothing, so that every step has the same loads in
-  // flight. A load's uniform offset never passes its buffer's end: the rows of a group past the last
-  // row are those of the first group again. All of it is selects and sums: a branch among the
-  // products would cost more than they do.
-  uint32_t wrow[LA], xrow[LB];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows
-    constexpr int Q = MODE == kRowsGateUp ? NA / 4 : 1;
-    const uint32_t r = MODE == kRowsGateUp ? (uint32_t)((i / Q & 1) * a.N + i / (2 * Q) * 8 * NA + i % Q * 32)
-                                           : 32u * i;
-    wrow[i] = __builtin_amdgcn_readfirstlane((int)r < wrows ? r * ldw : 0);
-  }
-#pragma unroll
-  for (int i = 0; i < LB; ++i)
-    xrow[i] = __builtin_amdgcn_readfirstlane(MODE != kRowsGateUp && 32 * i < ntok ? 32u * i * ldx : 0);
+  // flight. All of it is selects and sums: a branch among the products would cost more than they do.
   struct Step {
     uint32_t k0, stage;  // byte of K, LDS offset of the stage
     uint32_t off[2];     // kNowhere for the lanes past the row's end, else 0
@@ -374,6 +419,14 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   };
   constexpr int NLB = LB + (SC ? 1 : 0);
   constexpr int kB0 = S::kSA * S::kAStage;  // the token ring
+  // The first two steps' loads, in the order in which the steps issue them: tokens, then weights one
+  // further on (the third weights, whose stage the epilogue uses, are requested at the tile's start)
+  auto first_loads = [&]() __attribute__((always_inline)) {
+    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(0, 0), k); });
+    static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(0, kB0), k); });
+    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(1, S::kAStage), k); });
+    static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(1, kB0 + S::kBStage), k); });
+  };
 
   // ---- fragments
   const uint32_t lbase = lds_addr(lds);
@@ -400,13 +453,6 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   };
 
   f32x4_t acc[NA][NB];
-#pragma unroll
-  for (int x = 0; x < NA; ++x)
-#pragma unroll
-    for (int y = 0; y < NB; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int nblk = (ntok + 15) / 16;
-  const int nb = __builtin_amdgcn_readfirstlane(min(NB, (nblk - wn + 1) / 2));  // blocks with tokens
-
   Frag a0[HA], a1[HA], bx[HB], by[HB];
   uint32_t sx[HB] = {}, sy[HB] = {};
   auto ready_a = [&](Frag (&f)[HA]) __attribute__((always_inline)) {
@@ -439,7 +485,8 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
       tile_mma<ES, SC, H>(w[j], tk[i], sc[i], acc[X * HA + j][Y * HB + i]);
       __builtin_amdgcn_sched_barrier(0);
       static_for<NR>([&](auto k) __attribute__((always_inline)) {
-        if constexpr ((decltype(k)::value * RS < PROD ? decltype(k)::value * RS : PROD - 1) == p) read(k);
+        constexpr int due = decltype(k)::value * RS;
+        if constexpr ((due < PROD ? due : PROD - 1) == p) read(k);
       });
       static_for<NL>([&](auto k) __attribute__((always_inline)) {
         if constexpr (decltype(k)::value * PROD / NL + LO == p) load(k);
@@ -454,7 +501,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   const integral_constant<int, HB> chb{};
   const auto none = [](auto) {};
   // Ring offsets: the stages of this step and the next ones.
-  uint32_t ra[3] = {0, S::kAStage, 2 * S::kAStage}, rb[2] = {kB0, kB0 + S::kBStage};
+  uint32_t ra[3], rb[2];
   // Step d with its tokens' half 0 in p; half 1 goes to q, and the next step's half 0 after it.
   auto step = [&](int d, Frag (&p)[HB], uint32_t (&sp)[HB], Frag (&q)[HB], uint32_t (&sq)[HB])
                   __attribute__((always_inline)) {
@@ -465,95 +512,87 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     }, c0, none);
     lds_frags_ready();
     ready_b(q, sq);
+    wait_loads(LA + NLB);  // in flight: step d + 1's tokens, step d + 2's weights
+    __builtin_amdgcn_s_barrier();
+    const Step nb2 = step_b(d + 2, rb[0]), na3 = step_a(d + 3, ra[0]);
     quarter(a0, q, sq, c0, c1, cha, [&](auto k) __attribute__((always_inline)) {
       constexpr int K = decltype(k)::value;
       read_a(at, integral_constant<int, HA + K>{}, a1[K]);
-    }, c0, none);
+    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb2, k); });
     lds_frags_ready();
     ready_a(a1);
-    wait_loads(LA);  // step d + 2's weights may be in flight
-    __builtin_amdgcn_s_barrier();
-    const Step nb2 = step_b(d + 2, rb[0]), na3 = step_a(d + 3, ra[0]);
     quarter(a1, q, sq, c1, c1, cha, [&](auto k) __attribute__((always_inline)) {
       read_a(at1, k, a0[decltype(k)::value]);
-    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb2, k); });
+    }, c0, none);
+    lds_frags_ready();
+    ready_a(a0);
+    wait_loads(LA + NLB);  // in flight: step d + 2's weights and tokens
+    __builtin_amdgcn_s_barrier();
     quarter(a1, p, sp, c1, c0, chb, [&](auto k) __attribute__((always_inline)) {
       constexpr int K = decltype(k)::value;
       read_b(rb[1], k, q[K], sq[K]);
     }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na3, k); });
     lds_frags_ready();
-    ready_a(a0);
     ready_b(q, sq);
     const uint32_t t0 = ra[0], u0 = rb[0];
     ra[0] = ra[1], ra[1] = ra[2], ra[2] = t0;
     rb[0] = rb[1], rb[1] = u0;
   };
-  // A row's scale or pair, for the epilogue
-  uint32_t meta = 0;
-  if (tid < ntok) {
-    if (MODE == kRowsLinear)
-      meta = a.xs ? __float_as_uint(a.xs[t.r0 + tid]) : 0;
-    else
-      meta = a.order[t.r0 + tid];
-    if (MODE == kRowsGateUp) meta = __float_as_uint(a.xs[meta / a.topk]);
-  }
-  // (in the order in which the steps issue them: tokens, then weights one further on)
-  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(0, ra[0]), k); });
-  static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(0, rb[0]), k); });
-  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(1, ra[1]), k); });
-  static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(1, rb[1]), k); });
-  static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(2, ra[2]), k); });
-  wait_loads(2 * LA + NLB);  // step 0 has arrived
-  __builtin_amdgcn_s_barrier();
-  static_for<HA>([&](auto k) __attribute__((always_inline)) { read_a(aaddr, k, a0[decltype(k)::value]); });
-  static_for<HB>([&](auto k) __attribute__((always_inline)) {
-    constexpr int K = decltype(k)::value;
-    read_b(kB0, k, bx[K], sx[K]);
-  });
-  lds_frags_ready();
-  ready_a(a0);
-  ready_b(bx, sx);
-  for (int d = 0; d < nd; d += 2) {
-    step(d, bx, sx, by, sy);
-    step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
-  }
-  wait_loads(0);
-  mma_done(acc);
 
-  // ---- epilogue: half of the wave's token blocks at a time through LDS, row by row, so that one small
-  // loop serves all of the sums (unrolled over the registers it was 80 KB of instructions, which took
-  // longer to fetch than a tile of K = 1024 to multiply) and a row's outputs are stored together
-  constexpr int kStride = 16 * NA + 4;  // floats of a row: 16 bytes on, so that eight rows differ in banks
-  constexpr int kPart = HB * 16 * kStride;
-  static_assert(4 * kPart * 4 + S::kTRows * 4 <= S::kLds, "the waves' parts and the rows' values");
+  // ---- epilogue: a token block (16 rows) of a wave at a time through its quarter of a weight stage, so that
+  // one small loop serves all of the sums (unrolled over the registers it was 80 KB of instructions,
+  // which took longer to fetch than a tile of K = 1024 to multiply) and a row's outputs are stored
+  // together. Unit u of row r lies at unit u ^ (r & 7), so that eight rows differ in banks.
   constexpr int PER = (MODE == kRowsGateUp ? NA : 2 * NA);  // lanes of a row, eight outputs each
   constexpr int RPI = 64 / PER;
   static_assert(PER >= 4 && 64 % PER == 0 && 16 % (64 / PER) == 0, "whole turns in a token block");
   constexpr int UE = 16 / RPI;  // rows of a lane in a token block
-  float* part = reinterpret_cast<float*>(lds) + wave * kPart;
-  uint32_t* metas = reinterpret_cast<uint32_t*>(lds) + 4 * kPart;
+  constexpr int kRow = 16 * NA * 4;
+  static_assert(4 * 16 * kRow == S::kAStage, "the waves' quarters");
+  const uint32_t part = lbase + 2 * S::kAStage + wave * 16 * kRow;
   const int c = lane % PER, rsub = lane / PER;
-  const int n = n0 + wm * (S::kOut / 2) + c * 8;
-  float ws[8], other[8];  // scales, and the up scales or the bias
-  if constexpr (MODE == kRowsGateUp)
-    rows_gate_up_cols(a, t.e, n, ws, other);
-  else if constexpr (MODE == kRowsLinear)
-    rows_linear_cols(a, n, ws, other);
-  else
+  float ws[8], other[8], xs[NB];  // column scales, and the up scales or the bias; row scales
+  auto scales = [&](const Tile& t) __attribute__((always_inline)) {
+    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
+    if constexpr (MODE == kRowsGateUp) {
+      rows_gate_up_cols(a, t.e, n, ws, other);
+    } else if constexpr (MODE == kRowsLinear) {
+      rows_linear_cols(a, n, ws, other);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ws[i] = a.ws[(long long)t.e * a.N + min(n + i, a.N - 1)];
-  auto stage = [&](auto hc) __attribute__((always_inline)) {
-    constexpr int half = decltype(hc)::value;
+      for (int i = 0; i < 8; ++i) ws[i] = a.ws[(long long)t.e * a.N + min(n + i, a.N - 1)];
+      const int pair = a.order[t.r0 + min(tid, t.ntok - 1)];
+      if (tid < S::kTRows)
+        asm volatile("ds_write_b32 %0, %1" : : "v"(lbase + S::kMetas + tid * 4), "v"(pair) : "memory");
+    }
+    if constexpr (ES == 1 && MODE != kRowsDown) {
+      int row[NB];
 #pragma unroll
-    for (int i = 0; i < HB; ++i)
+      for (int b = 0; b < NB; ++b) row[b] = t.r0 + min((2 * b + wn) * 16 + lr, t.ntok - 1);
+      if constexpr (MODE == kRowsGateUp) {
 #pragma unroll
-      for (int x = 0; x < NA; ++x) {
-        const int col = MODE == kRowsGateUp && x >= HA ? 8 * NA + kq * SPAN + 4 * (x - HA)
-                                                       : kq * SPAN + 4 * x;
-        *reinterpret_cast<f32x4_t*>(part + (i * 16 + lr) * kStride + col) = acc[x][half * HB + i];
+        for (int b = 0; b < NB; ++b) row[b] = a.order[row[b]];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) row[b] /= a.topk;
       }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses run in order)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) xs[b] = a.xs[row[b]];
+    }
+  };
+  auto stage = [&](auto bc) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+    const uint32_t row = part + lr * kRow, key = lr & 7;
+#pragma unroll
+    for (int x = 0; x < NA; ++x) {
+      const int unit = MODE == kRowsGateUp && x >= HA ? 2 * NA + kq * (SPAN / 4) + x - HA
+                                                      : kq * (SPAN / 4) + x;
+      const uint32_t at = row + ((unit ^ key) * 16);
+      if constexpr (ES == 1 && MODE != kRowsDown) {
+        lds_write_scaled_sums(at, acc[x][b], xs[b]);
+      } else {
+        lds_write_sums(at, acc[x][b]);
+      }
+    }
   };
   // mul and residual of a token block. They are requested two blocks ahead and before the stores of the
   // block then at hand, because loads and stores complete in order: a load behind the stores would wait
@@ -562,51 +601,54 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   struct Ops {
     RowsOperands row[UE];
   };
-  const bool eight = n + 8 <= a.N;  // else some of the last columns, or none
   const uint16_t* idle = reinterpret_cast<const uint16_t*>(a.w);
   auto row_of = [&](int b, int i) __attribute__((always_inline)) {  // in the tile
     return (2 * b + wn) * 16 + rsub + i * RPI;
   };
-  auto fetch = [&](int b, Ops& o) __attribute__((always_inline)) {
+  auto fetch = [&](const Tile& t, int b, Ops& o) __attribute__((always_inline)) {
+    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
 #pragma unroll
     for (int i = 0; i < UE; ++i) {
       const int row = row_of(b, i);
-      const bool there = row < ntok && eight;
-      const long long at = (t.r0 + row) * a.N + n;
+      const bool there = row < t.ntok && n + 8 <= a.N;
+      const long long at = (long long)(t.r0 + row) * a.N + n;
       o.row[i].mul = rows_load8(a.mul && there ? a.mul + at : idle);
       o.row[i].res = rows_load8(a.res && there ? a.res + at : idle);
     }
   };
-  // Token block b. LDS is read by asm: before reads of its own the compiler would wait for the DMA
-  // loads, as which it counts the stores here too.
-  auto finish = [&](auto with, int b, Ops& o) __attribute__((always_inline)) {
+  // Token block b of the nb. LDS is accessed by asm: around accesses of its own the compiler would wait
+  // for the DMA loads, as which it counts the stores here too.
+  auto finish = [&](auto with, const Tile& t, int b, int nb, Ops& o) __attribute__((always_inline)) {
     constexpr bool WITH = decltype(with)::value;
-    if (b == HB) stage(c1);
-    const uint32_t src = lds_addr(part) + (((b < HB ? b : b - HB) * 16 + rsub) * kStride + c * 8) * 4;
-    const uint32_t msrc = lds_addr(metas) + row_of(b, 0) * 4;
+    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
+    static_for<NB>([&](auto k) __attribute__((always_inline)) {
+      if (b == decltype(k)::value) stage(k);
+    });
     u32x4v raw[UE][MODE == kRowsGateUp ? 4 : 2];
     uint32_t mv[UE];
-    static_for<UE>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value, off = i * RPI * kStride * 4;
-      raw[i][0] = lds_read_frag<off>(src);
-      raw[i][1] = lds_read_frag<off + 16>(src);
+#pragma unroll
+    for (int i = 0; i < UE; ++i) {
+      const int r = rsub + i * RPI;
+      const uint32_t at = part + r * kRow + ((2 * c) ^ (r & 7)) * 16;
+      raw[i][0] = lds_read_frag<0>(at);
+      raw[i][1] = lds_read_frag<0>(at ^ 16);
       if constexpr (MODE == kRowsGateUp) {
-        raw[i][2] = lds_read_frag<off + 32 * NA>(src);
-        raw[i][3] = lds_read_frag<off + 32 * NA + 16>(src);
+        raw[i][2] = lds_read_frag<32 * NA>(at);
+        raw[i][3] = lds_read_frag<32 * NA>(at ^ 16);
       }
-      mv[i] = lds_read4<i * RPI * 4>(msrc);
-    });
+      if constexpr (SC) mv[i] = lds_read4<0>(lbase + S::kMetas + row_of(b, i) * 4);
+    }
     lds_frags_ready();
 #pragma unroll
     for (int i = 0; i < UE; ++i) {
-      asm volatile("" : "+v"(mv[i]));
+      if (SC) asm volatile("" : "+v"(mv[i]));
 #pragma unroll
       for (u32x4v& f : raw[i]) after_wait(f);
     }
     uint4 w[UE];
 #pragma unroll
     for (int i = 0; i < UE; ++i) {
-      const bool live = row_of(b, i) < ntok;
+      const bool live = row_of(b, i) < t.ntok;
       const long long r = t.r0 + row_of(b, i);
       float v[8], u[8];
 #pragma unroll
@@ -615,43 +657,95 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
         if constexpr (MODE == kRowsGateUp) u[j] = __uint_as_float(raw[i][2 + j / 4][j % 4]);
       }
       if constexpr (MODE == kRowsGateUp) {
-        rows_gate_up_out(a, live, r, n, ws, other, __uint_as_float(mv[i]), v, u);
+        rows_gate_up_out(a, live, r, n, ws, other, v, u);
       } else if constexpr (MODE == kRowsDown) {
         rows_down_out(a, live, mv[i], n, ws, v);
       } else {
         RowsOperands op;
         if (WITH) {
           op = o.row[i];
-          if (live && n < a.N && !eight) rows_linear_load(a, r, n, op);
+          if (live && n < a.N && n + 8 > a.N) rows_linear_load(a, r, n, op);
         }
-        w[i] = rows_linear_value<WITH>(a, __uint_as_float(mv[i]), ws, other, op, v);
+        w[i] = rows_linear_value<WITH>(a, ws, other, op, v);
       }
     }
     if constexpr (MODE == kRowsLinear) {
-      if (WITH) fetch(min(b + 2, nb - 1), o);
+      if (WITH) fetch(t, min(b + 2, nb - 1), o);
 #pragma unroll
       for (int i = 0; i < UE; ++i)
-        if (row_of(b, i) < ntok && n < a.N)
+        if (row_of(b, i) < t.ntok && n < a.N)
           rows_linear_store<NA == 8>(a, t.r0 + row_of(b, i), n, w[i]);
     }
   };
-  __syncthreads();  // the stages have been read
-  if (tid < S::kTRows) metas[tid] = meta;
-  stage(c0);
-  __syncthreads();
-  if (nb <= 0) return;
-  Ops s0, s1;
-  if (MODE == kRowsLinear && (a.mul || a.res)) {
-    fetch(0, s0);
-    fetch(min(1, nb - 1), s1);
-#pragma unroll 1
-    for (int b = 0; b < nb; b += 2) {
-      finish(std::true_type{}, b, s0);
-      finish(std::true_type{}, b + 1, s1);  // (of no live rows if nb is odd)
+
+  set_sources(cur);
+  first_loads();
+  for (;;) {
+    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(2, 2 * S::kAStage), k); });
+    ra[0] = 0, ra[1] = S::kAStage, ra[2] = 2 * S::kAStage;
+    rb[0] = kB0, rb[1] = kB0 + S::kBStage;
+#pragma unroll
+    for (int x = 0; x < NA; ++x)
+#pragma unroll
+      for (int y = 0; y < NB; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    wait_loads(2 * LA + NLB);  // step 0 has arrived
+    __builtin_amdgcn_s_barrier();
+    static_for<HA>([&](auto k) __attribute__((always_inline)) { read_a(aaddr, k, a0[decltype(k)::value]); });
+    static_for<HB>([&](auto k) __attribute__((always_inline)) {
+      constexpr int K = decltype(k)::value;
+      read_b(kB0, k, bx[K], sx[K]);
+    });
+    lds_frags_ready();
+    ready_a(a0);
+    ready_b(bx, sx);
+    for (int d = 0; d < nd; d += 2) {
+      step(d, bx, sx, by, sy);
+      step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
     }
-  } else {
+    wait_loads(0);
+    mma_done(acc);
+    // What the epilogue reads is here before the next tile's loads are requested: behind them it would
+    // wait for them.
+    const int nb =
+        __builtin_amdgcn_readfirstlane(min(NB, ((cur.ntok + 15) / 16 - wn + 1) / 2));  // blocks with rows
+    Ops s0, s1;
+    const bool with = MODE == kRowsLinear && (a.mul || a.res) && nb > 0;
+    if (with) {
+      fetch(cur, 0, s0);
+      fetch(cur, min(1, nb - 1), s1);
+    }
+    id += gridDim.x;
+    const bool more = tile_of(id, next);
+    scales(cur);
+    if (more) set_sources(next);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(ws[i]), "+v"(other[i]));
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (ES == 1 && MODE != kRowsDown) asm volatile("" : "+v"(xs[b]));
+    if (with) {
+#pragma unroll
+      for (int i = 0; i < UE; ++i) {
+        tie(s0.row[i].mul), tie(s0.row[i].res);
+        tie(s1.row[i].mul), tie(s1.row[i].res);
+      }
+    }
+    __builtin_amdgcn_s_barrier();  // the stages have been read by all
+    if (more) first_loads();
+    if (with) {
 #pragma unroll 1
-    for (int b = 0; b < nb; ++b) finish(std::false_type{}, b, s0);
+      for (int b = 0; b < nb; b += 2) {
+        finish(std::true_type{}, cur, b, nb, s0);
+        finish(std::true_type{}, cur, b + 1, nb, s1);  // (of no live rows if nb is odd)
+      }
+    } else {
+#pragma unroll 1
+      for (int b = 0; b < nb; ++b) finish(std::false_type{}, cur, b, nb, s0);
+    }
+    if (!more) return;
+    __builtin_amdgcn_s_barrier();  // the third weight stage is free
+    cur = next;
   }
 }
 
@@ -790,16 +884,31 @@ hipError_t allow_tile_lds() {
   return err;
 }
 
+// Workgroups of the tile kernel that the device holds at once, by their LDS.
+int resident(int lds) {
+  static std::atomic<int> cus[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cus[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 8)
+      n = 256;
+    cus[dev].store(n, std::memory_order_relaxed);
+  }
+  return n / 8 * 8 * (160 * 1024 / lds);
+}
+
 template <int ES, int MODE, int NA, int NB>
 hipError_t launch_tile(const RowsGemm& a, hipStream_t s) {
   using S = TileShape<MODE, NA, NB>;
   const long long ncol = (a.N + S::kOut - 1) / S::kOut;
   const long long ntile = MODE == kRowsLinear ? (a.M + S::kTRows - 1) / S::kTRows : a.MT;
   if (ntile <= 0) return hipSuccess;
-  const long long grid = MODE == kRowsLinear ? (ncol * ntile + 7) / 8 * 8 : (ntile + 7) / 8 * 8 * ncol;
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  const long long tiles = MODE == kRowsLinear ? (ncol * ntile + 7) / 8 * 8 : (ntile + 7) / 8 * 8 * ncol;
+  if (tiles > 0x3fffffffLL) return hipErrorInvalidValue;
   hipError_t err = allow_tile_lds<ES, MODE, NA, NB>();
   if (err != hipSuccess) return err;
+  const long long grid = std::min<long long>(tiles, resident(S::kLds));
   hipLaunchKernelGGL((k_rows_tile<ES, MODE, NA, NB>), dim3((unsigned)grid), dim3(256), S::kLds, s, a,
                      (int)ncol, (int)ntile);
   return hipGetLastError();
