@@ -18,10 +18,11 @@ constexpr float kE4m3Max = 448.0f;
 __device__ __forceinline__ float row_scale(float amax) {
   return amax > 0.f ? fmaxf(amax, 0x1p-100f) / kE4m3Max : 1.0f;
 }
-// |v| where v is finite, else 0: what a row's amax is taken over.
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a < __builtin_inff() ? a : 0.f;
+// v, or NaN where v is not finite. A maximum with NaN is the other operand, so such values do not count
+// for an amax.
+__device__ __forceinline__ float finite_or_nan(float v) { return fmaf(v, 0.f, v); }
+__device__ __forceinline__ float amax_with(float amax, float v) {
+  return fmaxf(amax, fabsf(finite_or_nan(v)));
 }
 // v / s, correctly rounded, with r = 1 / s: the quotient's error is put back once, as a
 // division does. bf16 values fall on the middle between two e4m3 values often enough for the

@@ -18,7 +18,7 @@ __device__ __forceinline__ void store_row8(float (&v)[HC][8], int n, int lane, u
 #pragma unroll
   for (int c = 0; c < HC; ++c)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[c][j]));
+    for (int j = 0; j < 8; ++j) amax = amax_with(amax, v[c][j]);
   const float s = row_scale(wave_max(amax));
   const float r = 1.0f / s;
 #pragma unroll

@@ -978,7 +978,7 @@ Experts8Ws carve_experts8(void* base, int T, int H, int E, int k, int I) {
   Carver c{static_cast<char*>(base)};
   Experts8Ws w{};
   const int P = T * k;
-  w.bm = rows_tile_rows(T, k, E);
+  w.bm = rows_tile_rows(T, H, E, k, I);
   w.aq = c.take<uint8_t>((size_t)P * I);
   w.asc = c.take<uint8_t>((size_t)((I + 127) / 128) * P * 4);
   if (w.bm) {

@@ -6,7 +6,8 @@
 //                groups of 32 columns with one power-of-two scale each (the group format that
 //                the matrix instructions read, so the down product needs no pass of its own
 //                to find a row's amax, which no tile sees whole)
-//   kRowsDown    those groups times an expert's down rows: y[pair, n] = bf16(ws_n acc)
+//   kRowsDown    those groups times an expert's down rows: y[pair, n] = ws_n acc, in fp16 with a power
+//                of two for every 32 columns
 //
 // The kernels see rows of bytes. A step of K is 128 bytes of a row: lane (lr, kq) of a wave
 // holds the 16 bytes at 16 kq and the 16 at 64 + 16 kq of row lr, and feeds them to one
@@ -53,6 +54,7 @@ struct RowsGemm {
   const int* table;
   const int* order;
   int MT, topk;
+  int tile0;          // the first tile of a launch (few rows)
   long long P;        // pairs
   uint8_t* aq;        // [P, I] e4m3, in sorted order
   uint8_t* asc;       // [ceil(I / 128)][P][4]: biased exponent of each group of 32
@@ -95,6 +97,15 @@ __device__ __forceinline__ float rows_gate(float v, float t) {
                   fmaf(fmaf(x, kHalfL2e, -p), 0.693147182464599609375f, 1.0f);
   const float f = t < 0.f ? h : 1.0f;
   return v * f * f * __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
+}
+// silu with fewer instructions, v / (1 + exp(-v)): below v = -88 the result is 0 (its size is under
+// 10^-36, the least that an 8-bit group's scale can hold beside anything else).
+__device__ __forceinline__ float rows_silu(float v) {
+  constexpr float kL2e = -1.442695040888963407360f;
+  const float x = fminf(v, 200.f);  // v kL2e may overflow, and inf - inf is NaN
+  const float p = x * kL2e;
+  const float e = __builtin_amdgcn_exp2f(p) * fmaf(fmaf(x, kL2e, -p), 0.693147182464599609375f, 1.0f);
+  return v * __builtin_amdgcn_rcpf(1.0f + e);
 }
 // The activations, by the code that they share: relu and none; silu and gelu_tanh, v sigmoid(t) with
 // t = v or 2 sqrt(2 / pi) (v + 0.044715 v^3); gelu by erfc. (The sums 1 + tanh and 1 + erf would lose
@@ -202,33 +213,31 @@ __device__ __forceinline__ int group_exponent(float amax) {
 }
 // kRowsGateUp: columns n .. n + 7 of sorted row r, whose sums times the token's scale are g and u and
 // whose scales are sg and su; the four lanes of a group of 32 are neighbours. Every lane of the wave
-// calls; live: the row is stored. Scales of the groups that fill up the last 128 columns are
-// written as 1 (their values are read as zeros).
+// calls; live: the row is stored. The scales of groups behind the last one, whose values are read as
+// zeros, are written as 1.
 __device__ __forceinline__ void rows_gate_up_out(const RowsGemm& a, bool live, long long r, int n,
                                                  const float (&sg)[8], const float (&su)[8],
                                                  const float (&g)[8], const float (&u)[8]) {
   float v[8], amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float gv = g[i] * sg[i];
-    v[i] = rows_gate(gv, gv) * (u[i] * su[i]);
-    amax = fmaxf(amax, finite_abs(v[i]));
+    v[i] = finite_or_nan(rows_silu(g[i] * sg[i]) * (u[i] * su[i]));
+    amax = fmaxf(amax, fabsf(v[i]));
   }
   amax = fmaxf(amax, dppf<kDppXor1>(amax));
   amax = fmaxf(amax, dppf<kDppXor2>(amax));
   const int z = group_exponent(amax);
   const float m = __uint_as_float((uint32_t)(127 - z) << 23);
-  if (!live) return;
-  uint8_t* sc = a.asc + ((n >> 7) * a.P + r) * 4 + (n >> 5 & 3);
-  if (n >= a.N) {
-    *sc = 127;
-    return;
-  }
+  if (!live || n >= a.N) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], 0.f, v[i] * m);  // non-finite: NaN
+  for (int i = 0; i < 8; ++i) v[i] *= m;
   *reinterpret_cast<uint2*>(a.aq + r * a.N + n) =
       make_uint2(pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7]));
-  *sc = (uint8_t)(z + 127);  // all lanes of a group the same
+  uint8_t* sc = a.asc + ((n >> 7) * a.P + r) * 4;
+  const int grp = n >> 5;
+  sc[grp & 3] = (uint8_t)(z + 127);  // all lanes of a group the same
+  if (grp == a.N / 32 - 1)           // the groups that fill up the last 128 columns
+    for (int i = (grp & 3) + 1; i < 4; ++i) sc[i] = 127;
 }
 // The gate and up scales of columns n .. n + 7 of expert e.
 __device__ __forceinline__ void rows_gate_up_cols(const RowsGemm& a, int e, int n, float (&sg)[8],
@@ -249,7 +258,7 @@ __device__ __forceinline__ void rows_down_out(const RowsGemm& a, bool live, long
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[i] *= ws[i];
-    amax = fmaxf(amax, finite_abs(v[i]));
+    amax = amax_with(amax, v[i]);
   }
   amax = fmaxf(amax, dppf<kDppXor1>(amax));
   amax = fmaxf(amax, dppf<kDppXor2>(amax));
@@ -268,7 +277,7 @@ __device__ __forceinline__ void rows_down_out(const RowsGemm& a, bool live, long
 // es: bytes of an element. max_tiles: entries of the tile table at most (experts), built with
 // rows_tile_rows rows a tile. hipErrorInvalidValue for shapes outside the contract above.
 // rows_tile_rows 0: so few pairs that each is a tile of its own (ids in place of a table).
-int rows_tile_rows(int T, int k, int E);
+int rows_tile_rows(int T, int H, int E, int k, int I);
 hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_rows,
                             hipStream_t s);
 // kRowsDown and the weighted sum for tile_rows 0: out [T, N] = bf16(sum_j wts_tj ws acc).

@@ -1,6 +1,7 @@
 // Kernels of rows_gemm.h.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -10,7 +11,7 @@
 namespace moe {
 namespace {
 
-// The tile of weight block column blockIdx.x and tile blockIdx.y.
+// A tile's expert and rows.
 struct RowsTile {
   int e;
   long long r0, r1;  // token rows (kRowsLinear) or sorted pairs
@@ -44,7 +45,7 @@ template <int ES, int MODE, int NB, int MB, int W, int U>
 __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   __shared__ f32x4_t red[W][NB * MB][64];
   RowsTile t;
-  if (!rows_tile<MODE>(a, blockIdx.y, 16 * MB, t)) return;
+  if (!rows_tile<MODE>(a, a.tile0 + blockIdx.y, 16 * MB, t)) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, kq = lane >> 4;
@@ -163,10 +164,6 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= exs, u[j] *= exs;
     rows_gate_up_out(a, er < t.r1, er, en, ews, eother, v, u);
-    // the scales behind the last group
-    const int grp = blockIdx.x + 1 + ec;
-    if (blockIdx.x + 1 == gridDim.x && blockIdx.x % 4 + 1 + ec < 4 && er < t.r1)
-      a.asc[((grp >> 2) * a.P + er) * 4 + (grp & 3)] = 127;
   } else if constexpr (MODE == kRowsLinear) {
     if (a.xs) {
 #pragma unroll
@@ -849,21 +846,18 @@ hipError_t launch_few(const RowsGemm& a, hipStream_t s) {
   const long long tiles = MODE == kRowsLinear     ? (a.M + 16 * MB - 1) / (16 * MB)
                           : a.ids && !a.table ? a.P
                                               : a.MT;
-  if (tiles <= 0 || cols <= 0) return hipSuccess;
-  if (tiles > 65535 || cols > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W, U>), dim3((unsigned)cols, (unsigned)tiles),
-                     dim3(W * 64), 0, s, a);
-  return hipGetLastError();
-}
-template <int ES>
-hipError_t launch_few_linear(const RowsGemm& a, int mb, hipStream_t s) {
-  const char* e = getenv("ROWS_NB");
-  const int nb = e ? atoi(e) : a.N <= 4096 ? 1 : 2;
-  if (mb == 4) return launch_few<ES, kRowsLinear, 2, 4, 4, 2>(a, s);
-  if (mb == 2) return launch_few<ES, kRowsLinear, 2, 2, 8, 2>(a, s);
-  if (nb == 1) return launch_few<ES, kRowsLinear, 1, 1, 8, 4>(a, s);
-  if (nb == 3) return launch_few<ES, kRowsLinear, 1, 1, 8, 2>(a, s);
-  return launch_few<ES, kRowsLinear, 2, 1, 8, 2>(a, s);
+  if (cols > 0x7fffffffLL || tiles > 0x7fffffffLL) return hipErrorInvalidValue;
+  constexpr long long kGridY = 65535;
+  for (long long i = 0; i < tiles; i += kGridY) {
+    RowsGemm part = a;
+    part.tile0 = (int)i;
+    hipLaunchKernelGGL((k_rows_few<ES, MODE, NB, MB, W, U>),
+                       dim3((unsigned)cols, (unsigned)std::min(tiles - i, kGridY)), dim3(W * 64), 0, s,
+                       part);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 // A kernel's dynamic LDS above the default limit, allowed once per device.
@@ -924,21 +918,54 @@ bool tile_fits(RowsMode mode, const RowsGemm& a) {
   return (a.Kb + 127) / 128 * a.P * 4 < most;
 }
 
+// Up to 16 token rows one block of them, up to 32 two (K = 2048, kernel us at M = 32: N = 2048 bf16 6.8
+// as two workgroups of one block each, 10.1 as one of two, 10.9 by the 64 x 64 tile; N = 8192 e4m3 9.0,
+// 7.2, 8.4; at M = 64 that tile takes 8.9, two blocks 11.3). Of weight rows, 16 a workgroup up to
+// N = 4096, so that there are enough workgroups (one token, N = 2048 bf16: 5.5 us, 7.1 with 32), above
+// it 32, whose token loads are half (16 tokens, N = 8192 e4m3: 8.3, 9.1 with 16).
+//
+// Above that the tile of 64, 128 or 256 squared that takes the least time by its turns: a 256 tile has a
+// CU to itself and takes 54 us of K = 2048 bf16; of the smaller two or more share a CU, 17.5 and 7.7 us
+// each, at least one and 1.4 of them one after the other. (us, 64 / 128 / 256, K = 2048 bf16: 1024 x 2048
+// 17.3, 18.7, -; 2048 x 2048 30.7, 21.2, 48; 1024 x 8192 -, 38.8, 50.4; 2048 x 8192 -, 71.2, 58.7.)
 template <int ES>
-hipError_t launch_linear(const RowsGemm& a, int c, hipStream_t s) {
-  if (c == 256) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
-  if (c == 128) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
-  if (c == 64) return launch_tile<ES, kRowsLinear, 2, 2>(a, s);
-  return launch_few_linear<ES>(a, c ? c : 1, s);
+hipError_t launch_linear(const RowsGemm& a, hipStream_t s) {
+  const bool fits = tile_fits(kRowsLinear, a);
+  if (a.M <= 32 || !fits) {
+    if (a.N > 4096 && a.M > 16) return launch_few<ES, kRowsLinear, 2, 2, 8, 2>(a, s);
+    return a.N > 4096 ? launch_few<ES, kRowsLinear, 2, 1, 8, 2>(a, s)
+                      : launch_few<ES, kRowsLinear, 1, 1, 8, 4>(a, s);
+  }
+  auto turns = [&](long long b) {
+    return (double)(((a.M + b - 1) / b) * ((a.N + b - 1) / b)) / 256;
+  };
+  const double c64 = 7.7 * std::max(1.4, turns(64)), c128 = 17.5 * std::max(1.0, turns(128)),
+               c256 = 54 * std::ceil(turns(256));
+  if (c256 <= c128 && c256 <= c64) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
+  if (c128 <= c64) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
+  return launch_tile<ES, kRowsLinear, 2, 2>(a, s);
 }
 
 }  // namespace
 
-int rows_tile_rows(int T, int k, int E) {
+// Up to 16 pairs no tiles; else by the pairs r of an expert on average (us, H = 2048, I = 512, 256 experts,
+// tiles of 16 / 64 / 128 / 192 pairs: r = 4 162, 168, 186, 199; r = 16 253, 185, 207, 218; r = 32 398, 194,
+// 210, 225; r = 64 667, 251, 230, 246; r = 128 1185, 387, 325, 295). Tiles of 128 and 192 take a CU each
+// and 128 outputs of gate_up: where these are too few workgroups, 64 (8 experts, r = 256: 46 us, 56 with
+// 192; 16 experts of H = 4096, I = 1024, r = 128: 128 workgroups, 105 and 88).
+int rows_tile_rows(int T, int H, int E, int k, int I) {
   const long long P = (long long)T * k;
-  const char* e = getenv("ROWS_TILE");
-  if (e) return atoi(e);
-  return P <= 16 ? 0 : P > 12LL * E ? 192 : 16;
+  if (P <= 16) return 0;
+  RowsGemm gu{}, dn{};
+  gu.N = I, gu.ldw = gu.ldx = H, gu.xbytes = (long long)T * H;
+  dn.Kb = I, dn.ldw = dn.ldx = I, dn.P = P;
+  if (P <= 12LL * E || !tile_fits(kRowsGateUp, gu) || !tile_fits(kRowsDown, dn)) return 16;
+  auto workgroups = [&](long long rows) {
+    return (P + E * rows - 1) / (E * rows) * E * ((I + 127) / 128);
+  };
+  if (P <= 48LL * E) return 64;
+  const int rows = P <= 96LL * E ? 128 : 192;
+  return workgroups(rows) >= 128 ? rows : 64;
 }
 
 hipError_t launch_rows_pairs_down(const RowsGemm& a, int T, hipStream_t s) {
@@ -960,27 +987,23 @@ hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uin
 hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_rows,
                             hipStream_t s) {
   if (a.Kb < 16 || a.Kb % 16 || a.N < 1) return hipErrorInvalidValue;
-  if (mode == kRowsLinear) {
-    const char* e = getenv("ROWS_LIN");
-    int c = e ? atoi(e) : a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 64 ? 4 : 256;
-    if (!e && c == 256) {
-      auto n = [&](long long b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
-      c = n(256) >= 200 ? 256 : n(128) >= 128 ? 128 : 64;
-    }
-    if (!tile_fits(mode, a) && c > 4) c = 4;
-    return es == 2 ? launch_linear<2>(a, c, s) : launch_linear<1>(a, c, s);
-  }
+  if (mode == kRowsLinear) return es == 2 ? launch_linear<2>(a, s) : launch_linear<1>(a, s);
   if (es != 1 || a.N % 32) return hipErrorInvalidValue;
+  if (tile_rows > 16 && !tile_fits(mode, a)) return hipErrorInvalidValue;
   if (mode == kRowsGateUp) {
-    if (tile_rows == 192) return tile_fits(mode, a) ? launch_tile<1, kRowsGateUp, 8, 6>(a, s) : hipErrorInvalidValue;
-    return tile_rows <= 16   ? launch_few<1, kRowsGateUp, 4, 1, 4, 1>(a, s)
-           : tile_rows == 32 ? launch_few<1, kRowsGateUp, 4, 2, 8, 2>(a, s)
-                             : launch_few<1, kRowsGateUp, 4, 4, 4, 2>(a, s);
+    switch (tile_rows) {
+      case 64: return launch_tile<1, kRowsGateUp, 4, 2>(a, s);
+      case 128: return launch_tile<1, kRowsGateUp, 8, 4>(a, s);
+      case 192: return launch_tile<1, kRowsGateUp, 8, 6>(a, s);
+      default: return launch_few<1, kRowsGateUp, 4, 1, 4, 1>(a, s);
+    }
   }
-  if (tile_rows == 192) return tile_fits(mode, a) ? launch_tile<1, kRowsDown, 8, 6>(a, s) : hipErrorInvalidValue;
-  return tile_rows == 16   ? launch_few<1, kRowsDown, 2, 1, 4, 1>(a, s)
-         : tile_rows == 32 ? launch_few<1, kRowsDown, 4, 2, 4, 2>(a, s)
-                           : launch_few<1, kRowsDown, 2, 4, 4, 2>(a, s);
+  switch (tile_rows) {
+    case 64: return launch_tile<1, kRowsDown, 4, 2>(a, s);
+    case 128: return launch_tile<1, kRowsDown, 8, 4>(a, s);
+    case 192: return launch_tile<1, kRowsDown, 8, 6>(a, s);
+    default: return launch_few<1, kRowsDown, 2, 1, 4, 1>(a, s);
+  }
 }
 
 }  // namespace moe
