@@ -19,6 +19,8 @@ follows ``FastModel._moe``: bf16(w * y) for decode steps and for at most
 fp8-e4m3 experts: ``experts.gate_up_proj`` / ``down_proj`` of dtype float8_e4m3fn with
 per-output-row fp32 scales in ``experts.gate_up_scale`` [E, 2I] / ``experts.down_scale``
 [E, H] (see ``fp8.quantize_experts``).
+
+``add_rms_moe_fp8`` is ``add_rms_moe`` for such experts with 8-bit activations too.
 """
 
 from __future__ import annotations
@@ -27,7 +29,8 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr, stream_of
-from .ops import _need_cuda, expert_weight
+from .ops import (_need_cuda, add_rms_fp8, combine, expert_weight, experts_fp8, linear, route,
+                  router_logits)
 
 DECODE_EXPERT_TOKENS = 16  # engine/fast/model.py:48
 
@@ -129,6 +132,50 @@ def add_rms_moe(x: torch.Tensor, h: torch.Tensor | None, norm_weight: torch.Tens
     return out
 
 
+def add_rms_moe_fp8(x: torch.Tensor, h: torch.Tensor | None, norm_weight: torch.Tensor, eps: float,
+                    mlp, top_k: int, *, return_norm: bool = False, return_routing: bool = False):
+    """``add_rms_moe`` with the routed experts on 8-bit rows: ``ops.add_rms_fp8`` gives the norm as
+    e4m3 rows for ``ops.experts_fp8`` and as bf16 for the router and the shared expert
+    (``ops.linear``, its activation and product in the epilogues). Needs fp8 experts. Results
+    differ from ``add_rms_moe``'s by the rounding of the activations to e4m3, before each of the two
+    products; the routing is the same."""
+    shape = x.shape
+    x2 = _bf16_rows(x, "x")
+    h2 = None if h is None else _bf16_rows(h, "h").reshape(x2.shape)
+    gu, gus, dn, dns, wd = _expert_tensors(mlp.experts)
+    if wd != _lib.WEIGHTS_FP8_E4M3:
+        raise ValueError("add_rms_moe_fp8 needs float8_e4m3fn experts (see fp8.quantize_experts)")
+    sg, su, sd = _shared_weights(mlp.shared_expert)
+    pack = pack_router(mlp)
+    nexp = gu.shape[0]
+    total, q, scale, norm = add_rms_fp8(x2, h2, norm_weight.reshape(-1), float(eps), return_norm=True)
+    tokens, dev = x2.shape[0], x2.device
+    if not tokens:
+        new = lambda n, dtype: torch.empty((0, n), dtype=dtype, device=dev)  # noqa: E731
+        out, logits = torch.empty_like(x2), new(pack.shape[0], torch.bfloat16)
+        idx, wts = new(top_k, torch.long), new(top_k, torch.bfloat16)
+    else:
+        logits = router_logits(norm, pack)
+        wts, idx, _ = route(logits, top_k, nexp)
+        routed = experts_fp8(q, scale, idx, wts, gu, dn, gate_up_scale=gus, down_scale=dns)
+        act = linear(norm, su, mul=linear(norm, sg, activation="silu"))
+        one = torch.ones((tokens, 1), dtype=torch.bfloat16, device=dev)
+        out = combine(routed, one, shared=linear(act, sd), shared_gate_logit=logits[:, nexp],
+                      residual=total)
+    out = out.reshape(shape)
+    extra = (total.reshape(shape), norm.reshape(shape)) if return_norm else ()
+    extra += (idx, wts, logits) if return_routing else ()
+    return (out, *extra) if extra else out
+
+
+def _shared_weights(sh):
+    ws = (sh.gate_proj.weight, sh.up_proj.weight, sh.down_proj.weight)
+    for w, name in zip(ws, ("shared gate", "shared up", "shared down")):
+        if w.dtype != torch.bfloat16 or not w.is_contiguous():
+            raise ValueError(f"{name} weight must be contiguous bfloat16")
+    return ws
+
+
 def _bf16_rows(t: torch.Tensor, name: str) -> torch.Tensor:
     t2 = t.reshape(-1, t.shape[-1])
     _need_cuda(t2)
@@ -142,14 +189,8 @@ def _run(x2, mlp, top_k, decode, return_routing, residual=None, norm=None):
     gu, gus, dn, dns, wd = _expert_tensors(mlp.experts)
     experts, two_i, _ = gu.shape
     inter = two_i // 2
-    sh = mlp.shared_expert
-    sg = sh.gate_proj.weight
-    su = sh.up_proj.weight
-    sd = sh.down_proj.weight
+    sg, su, sd = _shared_weights(mlp.shared_expert)
     inter_s = sg.shape[0]
-    for w, name in ((sg, "shared gate"), (su, "shared up"), (sd, "shared down")):
-        if w.dtype != torch.bfloat16 or not w.is_contiguous():
-            raise ValueError(f"{name} weight must be contiguous bfloat16")
     pack = pack_router(mlp)
     n_pack = pack.shape[0]
     round_products = decode or tokens <= DECODE_EXPERT_TOKENS

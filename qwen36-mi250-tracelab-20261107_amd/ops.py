@@ -574,9 +574,9 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
     """Routed-expert output [T, H] bf16 for e4m3 rows ``q`` [T, H] with ``scale`` [T]
     (``add_rms_fp8``, ``quantize_rows``) and e4m3 experts (``fp8.quantize_experts``): both
     products on the e4m3 matrix instructions. Between them a = silu(gate) * up, fp32, goes in e4m3
-    with one power-of-two scale per 32 columns; pair outputs are rounded to bf16 and their weighted
-    sum, fp32 with bf16 weights, once more. ``top_k_index`` [T, k] int64 holds experts in
-    [0, E)."""
+    with one power-of-two scale per 32 columns. The pairs' outputs meet in fp32 (up to 16 pairs) or
+    through fp16 with a power of two per 32 columns; their weighted sum, fp32 with bf16 weights, is
+    rounded to bf16. ``top_k_index`` [T, k] int64 holds experts in [0, E)."""
     if not (q.is_cuda and gate_up.is_cuda and down.is_cuda and top_k_index.is_cuda):
         _need_cuda(q, gate_up, down, top_k_index)
     if q.dim() != 2:

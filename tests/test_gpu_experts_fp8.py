@@ -1,5 +1,4 @@
-"""ops.experts_fp8 against 64 bits, over shapes and routings, and the block that joins the 8-bit
-operators (block.add_rms_moe_fp8)."""
+"""ops.experts_fp8 against 64 bits, over shapes and routings."""
 
 from __future__ import annotations
 
