@@ -349,7 +349,10 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   // group past the last row are those of the first group again.
   __amdgpu_buffer_rsrc_t wbuf, xbuf, sbuf;
   uint32_t wrow[LA], xrow[LB], toff[MODE == kRowsGateUp ? LB : 1], soff;
+  int rot = 0;
   auto set_sources = [&](const Tile& t) __attribute__((always_inline)) {
+    if (MODE != kRowsLinear && ldw % 4096 == 0)
+      rot = (int)__umulhi((uint32_t)t.e * 2654435769u, (uint32_t)nd);
     const int wrows = MODE == kRowsGateUp ? 2 * a.N - t.n0 : min(S::kWRows, a.N - t.n0);
     wbuf = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(a.w + t.e * a.estride + (long long)t.n0 * a.ldw), 0,
@@ -391,14 +394,21 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     uint32_t k0, stage;  // byte of K, LDS offset of the stage
     uint32_t off[2];     // kNowhere for the lanes past the row's end, else 0
   };
-  auto past = [&](int d, uint32_t unit) __attribute__((always_inline)) {
-    return (uint32_t)d * 128 + unit < (uint32_t)a.Kb ? 0u : kNowhere;
+  auto byte_of = [&](int d) __attribute__((always_inline)) {
+    const int at = MODE == kRowsLinear ? d : d + rot;
+    return (uint32_t)min(MODE == kRowsLinear || at < nd ? at : at - nd, nd - 1) * 128;
+  };
+  auto past = [&](int d, uint32_t k0, uint32_t unit) __attribute__((always_inline)) {
+    if (MODE == kRowsLinear) return (uint32_t)d * 128 + unit < (uint32_t)a.Kb ? 0u : kNowhere;
+    return d < nd && k0 + unit < (uint32_t)a.Kb ? 0u : kNowhere;
   };
   auto step_a = [&](int d, uint32_t stage) __attribute__((always_inline)) {
-    return Step{(uint32_t)min(d, nd - 1) * 128, stage, {past(d, wunit[0]), past(d, wunit[1])}};
+    const uint32_t k0 = byte_of(d);
+    return Step{k0, stage, {past(d, k0, wunit[0]), past(d, k0, wunit[1])}};
   };
   auto step_b = [&](int d, uint32_t stage) __attribute__((always_inline)) {
-    return Step{(uint32_t)min(d, nd - 1) * 128, stage, {past(d, tunit), d < nd ? 0u : kNowhere}};
+    const uint32_t k0 = byte_of(d);
+    return Step{k0, stage, {past(d, k0, tunit), d < nd ? 0u : kNowhere}};
   };
   auto load_a = [&](const Step& st, auto ic) __attribute__((always_inline)) {
     constexpr int i = decltype(ic)::value;
