@@ -268,14 +268,20 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
 
 /* Routed experts on 8-bit rows q [T, H] with x_scale [T]: per pair (t, j) of top_k_index [T, k]
  * (each in [0, E)) a = silu(gate) * up in fp32, in e4m3 with one power-of-two scale per 32
- * columns (the least with amax <= 448 scale); y = bf16(a . down); out [T, H] =
- * bf16(sum_j top_k_weights[t, j] y_tj). gate_up [E, 2I, H] and down [E, H, I] are e4m3 with row
- * scales gu_scale [E, 2I] and dn_scale [E, H]; H and I multiples of 32, E <= 1024, k <= 64. */
+ * columns (the least with amax <= 448 scale); y = a . down, kept in fp32 for few pairs (16, or E / 4),
+ * else in fp16 with a power of two per 32 columns; out [T, H] = bf16(sum_j top_k_weights[t, j] y_tj).
+ * With shared [T, H] and its gate's logits (one bf16 per token, ld_gate elements apart) and with
+ * residual [T, H] (each may be null), out goes on as moe_combine does:
+ * bf16(bf16(out + bf16(bf16(sigmoid(gate)) * shared)) + residual).
+ * gate_up [E, 2I, H] and down [E, H, I] are e4m3 with row scales gu_scale [E, 2I] and dn_scale
+ * [E, H]; H and I multiples of 32, E <= 1024, k <= 64. q, the weights, shared, residual, out and
+ * the workspace are 16-byte aligned. */
 size_t moe_experts_fp8_workspace_bytes(int T, int H, int E, int k, int I);
 int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, int E, int k, int I,
                             const long long* top_k_index, const void* top_k_weights,
                             const void* gate_up, const float* gu_scale, const void* down,
-                            const float* dn_scale, void* out, void* workspace,
+                            const float* dn_scale, const void* shared, const void* shared_gate,
+                            long long ld_gate, const void* residual, void* out, void* workspace,
                             size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

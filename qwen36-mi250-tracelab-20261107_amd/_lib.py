@@ -83,7 +83,7 @@ SIGNATURES: dict[str, tuple] = {
         _I, [_P, _LL, _P, _P, _LL, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P, _P]),
     "moe_experts_fp8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "moe_experts_fp8_forward": (
-        _I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+        _I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P, _P, _P, _SZ, _P]),
 }
 
 

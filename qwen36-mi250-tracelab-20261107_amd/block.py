@@ -29,7 +29,7 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr, stream_of
-from .ops import (_need_cuda, add_rms_fp8, combine, expert_weight, experts_fp8, linear, route,
+from .ops import (_call, _need_cuda, add_rms_fp8, expert_weight, experts_fp8, linear,
                   router_logits)
 
 DECODE_EXPERT_TOKENS = 16  # engine/fast/model.py:48
@@ -156,16 +156,24 @@ def add_rms_moe_fp8(x: torch.Tensor, h: torch.Tensor | None, norm_weight: torch.
         idx, wts = new(top_k, torch.long), new(top_k, torch.bfloat16)
     else:
         logits = router_logits(norm, pack)
-        wts, idx, _ = route(logits, top_k, nexp)
-        routed = experts_fp8(q, scale, idx, wts, gu, dn, gate_up_scale=gus, down_scale=dns)
+        wts, idx = _route(logits, top_k, nexp)
         act = linear(norm, su, mul=linear(norm, sg, activation="silu"))
-        one = torch.ones((tokens, 1), dtype=torch.bfloat16, device=dev)
-        out = combine(routed, one, shared=linear(act, sd), shared_gate_logit=logits[:, nexp],
-                      residual=total)
+        out = experts_fp8(q, scale, idx, wts, gu, dn, gate_up_scale=gus, down_scale=dns,
+                          shared=linear(act, sd), shared_gate_logit=logits[:, nexp], residual=total)
     out = out.reshape(shape)
     extra = (total.reshape(shape), norm.reshape(shape)) if return_norm else ()
     extra += (idx, wts, logits) if return_routing else ()
     return (out, *extra) if extra else out
+
+
+def _route(logits, top_k, experts):
+    """``ops.route`` without the counts of pairs, which ``ops.experts_fp8`` makes for itself."""
+    tokens = logits.shape[0]
+    wts = torch.empty((tokens, top_k), dtype=torch.bfloat16, device=logits.device)
+    idx = torch.empty((tokens, top_k), dtype=torch.long, device=logits.device)
+    _call("route", logits.get_device(), _lib.load().moe_route_topk, ptr(logits), logits.stride(0), tokens,
+          experts, top_k, ptr(idx), ptr(wts), None)
+    return wts, idx
 
 
 def _shared_weights(sh):

@@ -1217,22 +1217,31 @@ size_t moe_experts_fp8_workspace_bytes(int T, int H, int E, int k, int I) {
 int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, int E, int k, int I,
                             const long long* top_k_index, const void* top_k_weights,
                             const void* gate_up, const float* gu_scale, const void* down,
-                            const float* dn_scale, void* out, void* workspace,
-                            size_t workspace_bytes, void* stream) {
+                            const float* dn_scale, const void* shared,
+                            const void* shared_gate, long long ld_gate, const void* residual,
+                            void* out, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_experts_shape(T, H, E, k, I);
   if (rc) return rc;
   if (T == 0) return MOE_OK;
   CHECK_ARG(q && x_scale && top_k_index && top_k_weights && gate_up && gu_scale && down &&
                 dn_scale && out,
             "experts_fp8: null pointer");
-  CHECK_ARG(((uintptr_t)q | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)out |
-             (uintptr_t)workspace) % 16 == 0,
-            "experts_fp8: q, the weights, out and the workspace must be 16-byte aligned");
+  CHECK_ARG(!shared || (shared_gate && ld_gate >= 0), "experts_fp8: shared needs its gate's logits");
+  CHECK_ARG(((uintptr_t)q | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)shared |
+             (uintptr_t)residual | (uintptr_t)out | (uintptr_t)workspace) % 16 == 0,
+            "experts_fp8: q, the weights, shared, residual, out and the workspace must be 16-byte aligned");
+  const long long row = 2LL * T * H;
+  const Span in[] = {{q, row / 2}, {shared, row}, {residual, row}};
+  const Span o{out, row};
+  CHECK_ARG(apart(in, 3, &o, 1), "experts_fp8: out must not overlap the inputs");
   const Experts8Ws w = carve_experts8(workspace, T, H, E, k, I);
   CHECK_ARG(workspace && workspace_bytes >= w.bytes, "experts_fp8: workspace too small: %zu < %zu",
             workspace_bytes, w.bytes);
   hipStream_t s = (hipStream_t)stream;
   const uint16_t* wts = static_cast<const uint16_t*>(top_k_weights);
+  const RowsTail tail{static_cast<const uint16_t*>(shared),
+                      static_cast<const uint16_t*>(shared_gate),
+                      static_cast<const uint16_t*>(residual), ld_gate};
   RowsGemm a{};
   a.x = static_cast<const uint8_t*>(q), a.ldx = H, a.xbytes = (long long)T * H;
   a.w = static_cast<const uint8_t*>(gate_up), a.ldw = H, a.estride = 2LL * I * H;
@@ -1256,11 +1265,12 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
   a.N = H, a.Kb = I;
   if (!w.bm) {
     a.out = static_cast<uint16_t*>(out), a.wts = wts;
-    return hip_check(launch_rows_pairs_down(a, T, s), "down launch");
+    return hip_check(launch_rows_pairs_down(a, tail, T, s), "down launch");
   }
   a.out = w.y, a.yexp = w.yexp;
   HIP_TRY(launch_rows_gemm(kRowsDown, 1, a, w.bm, s), "down launch");
-  return hip_check(launch_rows_combine(w.y, w.yexp, wts, T, H, k, static_cast<uint16_t*>(out), s),
+  return hip_check(launch_rows_combine(w.y, w.yexp, wts, tail, T, H, k, static_cast<uint16_t*>(out),
+                                       s),
                    "combine launch");
 }
 

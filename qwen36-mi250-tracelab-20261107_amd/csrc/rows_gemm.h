@@ -64,6 +64,21 @@ struct RowsGemm {
   const uint16_t* wts;
 };
 
+// What a layer adds to the routed sum, rounded as the block's combine rounds it: bf16(sum), then
+// bf16(. + bf16(bf16(sigmoid(gate_t)) shared)), then + residual. Null: not there.
+struct RowsTail {
+  const uint16_t *shared, *gate, *res;  // [T, H], one per token ld_gate apart, [T, H]
+  long long ld_gate;
+};
+__device__ __forceinline__ float rows_tail_gate(const RowsTail& t, long long row) {
+  return t.shared ? rbf(sigmoidf_(bf_bits2f(t.gate[row * t.ld_gate]))) : 0.f;
+}
+__device__ __forceinline__ float rows_tail(const RowsTail& t, float sum, float gate, float shared,
+                                           float res) {
+  if (t.shared) sum = rbf(rbf(sum) + rbf(gate * shared));
+  return t.res ? rbf(sum) + res : sum;
+}
+
 typedef int v8i_t __attribute__((ext_vector_type(8)));
 
 // One 128-byte step of K: acc += W (a0 | a1) . X (b0 | b1).
@@ -280,10 +295,11 @@ __device__ __forceinline__ void rows_down_out(const RowsGemm& a, bool live, long
 int rows_tile_rows(int T, int H, int E, int k, int I);
 hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_rows,
                             hipStream_t s);
-// kRowsDown and the weighted sum for tile_rows 0: out [T, N] = bf16(sum_j wts_tj ws acc).
-hipError_t launch_rows_pairs_down(const RowsGemm& a, int T, hipStream_t s);
-// out [T, H] = bf16(sum_j w_tj y_tj) for y as kRowsDown writes it.
-hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w, int T, int H,
-                               int k, uint16_t* out, hipStream_t s);
+// kRowsDown and the weighted sum for tile_rows 0: out [T, N] = bf16(sum_j wts_tj ws acc) and the tail.
+hipError_t launch_rows_pairs_down(const RowsGemm& a, const RowsTail& tail, int T, hipStream_t s);
+// out [T, H] = bf16(sum_j w_tj y_tj) and the tail, for y as kRowsDown writes it.
+hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w,
+                               const RowsTail& tail, int T, int H, int k, uint16_t* out,
+                               hipStream_t s);
 
 }  // namespace moe

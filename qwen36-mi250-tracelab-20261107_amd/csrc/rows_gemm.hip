@@ -759,7 +759,8 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
 // The down product of a few pairs and their weighted sum: 16 outputs of one token a workgroup, a wave
 // a pair.
 constexpr int kPairWaves = 8;
-__global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a) {
+__global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a,
+                                                                    RowsTail tail) {
   __shared__ float part[kPairWaves][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -805,24 +806,32 @@ __global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[wave][4 * kq + i] = total[i];
   }
-  __syncthreads();
   const int n = threadIdx.x;
+  const long long at = (long long)blockIdx.y * a.N + n0 + (n & 15);
+  const float gate = rows_tail_gate(tail, blockIdx.y);
+  const float shared = tail.shared ? bf_bits2f(tail.shared[at]) : 0.f;
+  const float res = tail.res ? bf_bits2f(tail.res[at]) : 0.f;
+  __syncthreads();
   if (n >= 16) return;
   float s = part[0][n];
 #pragma unroll
   for (int w = 1; w < kPairWaves; ++w) s += part[w][n];
-  a.out[(long long)blockIdx.y * a.N + n0 + n] = f2bf_bits(s);
+  a.out[at] = f2bf_bits(rows_tail(tail, s, gate, shared, res));
 }
 
 // Eight outputs a thread, the pairs' values of eight pairs requested together. Bound by memory.
 __global__ __launch_bounds__(256) void k_rows_combine(const uint16_t* y, const uint8_t* yexp,
-                                                      const uint16_t* w, int T, int H, int k,
-                                                      uint16_t* out) {
+                                                      const uint16_t* w, RowsTail tail, int T, int H,
+                                                      int k, uint16_t* out) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   const int per = H / 8;
   const long long t = i / per;
   if (t >= T) return;
   const int c = (int)(i - t * per) * 8;
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+  const uint4 sh = tail.shared ? ld16_stream(tail.shared + t * H + c) : none;
+  const uint4 rs = tail.res ? ld16_stream(tail.res + t * H + c) : none;
+  const float gate = rows_tail_gate(tail, t);
   float acc[8] = {};
   for (int j0 = 0; j0 < k; j0 += 8) {
     uint4 v[8];
@@ -845,6 +854,12 @@ __global__ __launch_bounds__(256) void k_rows_combine(const uint16_t* y, const u
         acc[2 * x + 1] = fmaf((float)h[1], m[j], acc[2 * x + 1]);
       }
     }
+  }
+  const uint32_t su[4] = {sh.x, sh.y, sh.z, sh.w}, ru[4] = {rs.x, rs.y, rs.z, rs.w};
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    acc[2 * x] = rows_tail(tail, acc[2 * x], gate, bf_lo(su[x]), bf_lo(ru[x]));
+    acc[2 * x + 1] = rows_tail(tail, acc[2 * x + 1], gate, bf_hi(su[x]), bf_hi(ru[x]));
   }
   st16(out + t * H + c, make_uint4(pack_bf2_rne(acc[0], acc[1]), pack_bf2_rne(acc[2], acc[3]),
                                    pack_bf2_rne(acc[4], acc[5]), pack_bf2_rne(acc[6], acc[7])));
@@ -958,14 +973,16 @@ hipError_t launch_linear(const RowsGemm& a, hipStream_t s) {
 
 }  // namespace
 
-// Up to 16 pairs no tiles; else by the pairs r of an expert on average (us, H = 2048, I = 512, 256 experts,
-// tiles of 16 / 64 / 128 / 192 pairs: r = 4 162, 168, 186, 199; r = 16 253, 185, 207, 218; r = 32 398, 194,
+// Up to 16 pairs, or one for every four experts, no tiles: few share an expert, and there is nothing to
+// sort (us, H = 2048, I = 512, 256 experts, each pair by itself / tiles of 16: 32 pairs 25, 34; 64 41,
+// 50; 128 75, 74; 16 experts of H = 4096, I = 1024: 32 pairs 79, 48). Else by the pairs r of an expert on
+// average (256 experts as above, tiles of 16 / 64 / 128 / 192 pairs: r = 4 162, 168, 186, 199; r = 16 253, 185, 207, 218; r = 32 398, 194,
 // 210, 225; r = 64 667, 251, 230, 246; r = 128 1185, 387, 325, 295). Tiles of 128 and 192 take a CU each
 // and 128 outputs of gate_up: where these are too few workgroups, 64 (8 experts, r = 256: 46 us, 56 with
 // 192; 16 experts of H = 4096, I = 1024, r = 128: 128 workgroups, 105 and 88).
 int rows_tile_rows(int T, int H, int E, int k, int I) {
   const long long P = (long long)T * k;
-  if (P <= 16) return 0;
+  if (P <= std::max(16, E / 4)) return 0;
   RowsGemm gu{}, dn{};
   gu.N = I, gu.ldw = gu.ldx = H, gu.xbytes = (long long)T * H;
   dn.Kb = I, dn.ldw = dn.ldx = I, dn.P = P;
@@ -978,19 +995,21 @@ int rows_tile_rows(int T, int H, int E, int k, int I) {
   return workgroups(rows) >= 128 ? rows : 64;
 }
 
-hipError_t launch_rows_pairs_down(const RowsGemm& a, int T, hipStream_t s) {
+hipError_t launch_rows_pairs_down(const RowsGemm& a, const RowsTail& tail, int T, hipStream_t s) {
   if (T <= 0) return hipSuccess;
   if (T > 65535 || a.N % 32 || a.Kb < 16 || a.Kb % 16) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(k_rows_pairs_down, dim3(a.N / 16, T), dim3(kPairWaves * 64), 0, s, a);
+  hipLaunchKernelGGL(k_rows_pairs_down, dim3(a.N / 16, T), dim3(kPairWaves * 64), 0, s, a, tail);
   return hipGetLastError();
 }
 
-hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w, int T, int H,
-                               int k, uint16_t* out, hipStream_t s) {
+hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uint16_t* w,
+                               const RowsTail& tail, int T, int H, int k, uint16_t* out,
+                               hipStream_t s) {
   if (T <= 0) return hipSuccess;
   const long long grid = ((long long)T * (H / 8) + 255) / 256;
   if (H % 32 || grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)grid), dim3(256), 0, s, y, yexp, w, T, H, k, out);
+  hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)grid), dim3(256), 0, s, y, yexp, w, tail, T, H, k,
+                     out);
   return hipGetLastError();
 }
 

@@ -570,13 +570,16 @@ def _rows_in_place(t: torch.Tensor, k: int, size: int) -> bool:
 
 def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
                 top_k_weights: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, *,
-                gate_up_scale: torch.Tensor, down_scale: torch.Tensor) -> torch.Tensor:
+                gate_up_scale: torch.Tensor, down_scale: torch.Tensor,
+                shared: torch.Tensor | None = None, shared_gate_logit: torch.Tensor | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
     """Routed-expert output [T, H] bf16 for e4m3 rows ``q`` [T, H] with ``scale`` [T]
     (``add_rms_fp8``, ``quantize_rows``) and e4m3 experts (``fp8.quantize_experts``): both
     products on the e4m3 matrix instructions. Between them a = silu(gate) * up, fp32, goes in e4m3
-    with one power-of-two scale per 32 columns. The pairs' outputs meet in fp32 (up to 16 pairs) or
-    through fp16 with a power of two per 32 columns; their weighted sum, fp32 with bf16 weights, is
-    rounded to bf16. ``top_k_index`` [T, k] int64 holds experts in [0, E)."""
+    with one power-of-two scale per 32 columns. The pairs' outputs meet in fp32 (few pairs) or through
+    fp16 with a power of two per 32 columns; their weighted sum, fp32 with bf16 weights, is
+    rounded to bf16. ``top_k_index`` [T, k] int64 holds experts in [0, E). ``shared`` [T, H] with
+    ``shared_gate_logit`` [T] and ``residual`` [T, H], bf16, are added as ``combine`` adds them."""
     if not (q.is_cuda and gate_up.is_cuda and down.is_cuda and top_k_index.is_cuda):
         _need_cuda(q, gate_up, down, top_k_index)
     if q.dim() != 2:
@@ -607,6 +610,18 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
     dns = _vector(down_scale, _F32, "down_scale", nexp * hidden, dev)
     idx = top_k_index if top_k_index.is_contiguous() else top_k_index.contiguous()
     wts = top_k_weights.to(torch.bfloat16).contiguous()
+    ld_gate = 0
+    if shared is not None:
+        if shared.shape != q.shape or shared_gate_logit is None or shared_gate_logit.shape != (tokens,):
+            raise ValueError(f"shared must be {tuple(q.shape)} and shared_gate_logit [{tokens}]")
+        shared = _input(shared, torch.bfloat16, "shared", dev)
+        if shared_gate_logit.dtype is not torch.bfloat16 or shared_gate_logit.get_device() != dev:
+            raise ValueError(f"shared_gate_logit must be bfloat16 on {q.device}")
+        ld_gate = shared_gate_logit.stride(0)
+    if residual is not None:
+        if residual.shape != q.shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, the output {tuple(q.shape)}")
+        residual = _input(residual, torch.bfloat16, "residual", dev)
     out = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=q.device)
     lib = _lib.load()
     nbytes = lib.moe_experts_fp8_workspace_bytes(tokens, hidden, nexp, top_k, inter)
@@ -614,5 +629,7 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
     _call("experts_fp8", dev, lib.moe_experts_fp8_forward, q.data_ptr(), scale.data_ptr(), tokens,
           hidden, nexp, top_k, inter, idx.data_ptr(), wts.data_ptr(), gate_up.data_ptr(),
-          gus.data_ptr(), down.data_ptr(), dns.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
+          gus.data_ptr(), down.data_ptr(), dns.data_ptr(), ptr(shared),
+          None if shared is None else shared_gate_logit.data_ptr(), ld_gate, ptr(residual),
+          out.data_ptr(), ws.data_ptr(), nbytes)
     return out

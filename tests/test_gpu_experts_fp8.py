@@ -139,3 +139,29 @@ def test_experts_fp8_refusals(pkg, dev):
                     ("down_scale", good["down_scale"].double()), ("scale", good["scale"].cpu())):
         with pytest.raises((ValueError, pkg.MoeLibraryError)):
             pkg.ops.experts_fp8(**{**good, name: t})
+
+
+@pytest.mark.parametrize("E", [8, 200])
+@pytest.mark.parametrize("T", [1, 5, 40, 300])
+def test_experts_fp8_with_shared_and_residual_is_combine(pkg, dev, T, E):
+    q, xs, gu, gus, dn, dns, g = _layer(T, 96, E, 64, T + 20)
+    idx, wts = routing(T, E, 4, "uniform", g)
+    shared, res = (torch.randn(T, 96, generator=g).to(BF16).to(dev) for _ in range(2))
+    gate = (torch.randn(T, 7, generator=g) * 4).to(BF16).to(dev)[:, 3]
+    args = [t.to(dev) for t in (q, xs, idx, wts, gu, dn)]
+    call = lambda **kw: pkg.ops.experts_fp8(*args, gate_up_scale=gus.to(dev), down_scale=dns.to(dev), **kw)  # noqa: E731
+    routed, one = call(), torch.ones(T, 1, dtype=BF16, device=dev)
+    for s, r in ((None, res), (shared, None), (shared, res)):
+        want = pkg.ops.combine(routed, one, shared=s, shared_gate_logit=None if s is None else gate, residual=r)
+        kw = {} if s is None else dict(shared=s, shared_gate_logit=gate)
+        assert torch.equal(call(residual=r, **kw), want)
+    wide = torch.zeros(T, 200, dtype=BF16, device=dev)  # views, one at an odd address
+    wide[:, 5:101], wide[:, 104:] = shared, res
+    assert torch.equal(call(shared=wide[:, 5:101], shared_gate_logit=gate.contiguous(), residual=wide[:, 104:]),
+                       call(shared=shared, shared_gate_logit=gate, residual=res))
+    for bad in (dict(shared=shared), dict(shared=shared, shared_gate_logit=gate[:-1]), dict(residual=res[:, :64]),
+                dict(shared=shared[:, :64], shared_gate_logit=gate), dict(residual=res.float()),
+                dict(shared=shared, shared_gate_logit=gate.float()), dict(shared=shared, shared_gate_logit=gate[:, None]),
+                dict(residual=res.cpu())):
+        with pytest.raises((ValueError, pkg.MoeLibraryError)):
+            call(**bad)

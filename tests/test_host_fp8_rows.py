@@ -82,8 +82,9 @@ def test_experts_fp8_refusals(pkg):
     assert 0 < need < lib.moe_experts_fp8_workspace_bytes(400, 64, 8, 2, 32)
     assert lib.moe_experts_fp8_workspace_bytes(-1, 64, 8, 2, 32) == 0
 
-    def call(q=A, xs=B, T=4, H=64, E=8, k=2, I=32, idx=B, wts=B, gu=B, gus=B, dn=B, dns=B, out=C, ws=D, n=need):
-        return f(q, xs, T, H, E, k, I, idx, wts, gu, gus, dn, dns, out, ws, n, None)
+    def call(q=A, xs=B, T=4, H=64, E=8, k=2, I=32, idx=B, wts=B, gu=B, gus=B, dn=B, dns=B, out=C, ws=D, n=need,
+             sh=None, gate=None, ld=1, res=None):
+        return f(q, xs, T, H, E, k, I, idx, wts, gu, gus, dn, dns, sh, gate, ld, res, out, ws, n, None)
 
     _refused(pkg, call(H=40), b"hidden")
     _refused(pkg, call(I=48), b"intermediate")
@@ -96,6 +97,12 @@ def test_experts_fp8_refusals(pkg):
     _refused(pkg, call(q=A + 8), b"aligned")
     _refused(pkg, call(n=need - 1), b"workspace")
     _refused(pkg, call(ws=None), b"workspace")
+    _refused(pkg, call(sh=B), b"gate")
+    _refused(pkg, call(sh=B, gate=B, ld=-1), b"gate")
+    _refused(pkg, call(sh=B + 4, gate=B), b"aligned")
+    _refused(pkg, call(res=B + 8), b"aligned")
+    _refused(pkg, call(res=C), b"overlap")
+    _refused(pkg, call(sh=C + 64, gate=B), b"overlap")
     assert call(T=0, q=None) == 0
 
 
