@@ -273,9 +273,10 @@ __device__ __forceinline__ void dma4_buffer(__amdgpu_buffer_rsrc_t buf, void* ld
   __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void*)lds, 4, voff, soff, 0, 0);
 }
 
-template <int MODE, int NA, int NB>
+template <int MODE, int NA, int NB, int W>
 struct TileShape {
-  static constexpr int kWRows = 32 * NA, kTRows = 32 * NB;
+  static constexpr int kWM = W / 2;  // waves side by side along the weight rows
+  static constexpr int kWRows = 16 * NA * kWM, kTRows = 32 * NB;
   static constexpr int kSA = 3, kSB = 2;
   static constexpr bool kScaled = MODE == kRowsDown;
   static constexpr int kAStage = kWRows * 128;
@@ -286,16 +287,16 @@ struct TileShape {
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
-template <int ES, int MODE, int NA, int NB>
-__global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int ntile) {
-  using S = TileShape<MODE, NA, NB>;
+template <int ES, int MODE, int NA, int NB, int W>
+__global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, int ntile) {
+  using S = TileShape<MODE, NA, NB, W>;
   constexpr bool SC = S::kScaled;
   constexpr int HA = NA / 2, HB = NB / 2;
-  constexpr int LA = S::kWRows / 32, LB = S::kTRows / 32;  // loads of a wave and step
+  constexpr int LA = S::kWRows / (8 * W), LB = S::kTRows / (8 * W);  // loads of a wave and step
   extern __shared__ uint4 smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave % S::kWM, wn = wave / S::kWM;
   const int lr = lane & 15, kq = lane >> 4;
   char* lds = reinterpret_cast<char*>(smem);
 
@@ -332,14 +333,17 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   // ---- DMA: the wave's load i fills LDS rows (wave + 4 i) 8 .. + 7, lane l unit l & 7 of row l >> 3
   constexpr uint32_t kNowhere = 0x80000000u;  // past the end of any of the buffers
   constexpr int SPAN = MODE == kRowsGateUp ? 2 * NA : 4 * NA;
+  // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows; UP: both in one load of the waves
+  constexpr bool UP = MODE == kRowsGateUp && W > NA;
+  static_assert(!UP || W == 2 * NA, "the waves' load is a wm's rows");
   const int grow = lane >> 3, row0 = wave * 8 + grow;
   const uint32_t ldw = (uint32_t)a.ldw, ldx = (uint32_t)a.ldx;
   uint32_t wunit[2], woff[2];  // by load parity (the key of row0 + 32)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = row0 + 32 * i, key = (r & 3) | (((r / SPAN) & 1) << 2);
+    const int r = row0 + 8 * W * i, key = (r & 3) | (((r / SPAN) & 1) << 2);
     wunit[i] = ((lane & 7) ^ key) * 16;
-    woff[i] = row0 * ldw + wunit[i];
+    woff[i] = (UP ? row0 % (8 * NA) : row0) * ldw + wunit[i];
   }
   const uint32_t tunit = ((lane & 7) ^ grow) * 16;
   // (the last wave's scale load, past the stage's rows, repeats the one before)
@@ -367,22 +371,21 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     soff = srow + lane < t.ntok ? (srow + lane) * 4 : kNowhere;
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
-      // kRowsGateUp's LDS rows: per wm 8 NA gate rows, then their up rows
-      constexpr int Q = MODE == kRowsGateUp ? NA / 4 : 1;
-      const uint32_t r = MODE == kRowsGateUp
-                             ? (uint32_t)((i / Q & 1) * a.N + i / (2 * Q) * 8 * NA + i % Q * 32)
-                             : 32u * i;
+      constexpr int Q = MODE == kRowsGateUp && !UP ? NA / W : 1;
+      const uint32_t r = UP                    ? (uint32_t)(wave / NA * a.N + i * 8 * NA)
+                         : MODE == kRowsGateUp ? (uint32_t)((i / Q & 1) * a.N + i / (2 * Q) * 8 * NA + i % Q * 8 * W)
+                                               : 8u * W * i;
       wrow[i] = __builtin_amdgcn_readfirstlane((int)r < wrows ? r * ldw : 0);
     }
 #pragma unroll
     for (int i = 0; i < LB; ++i)
       xrow[i] =
-          __builtin_amdgcn_readfirstlane(MODE != kRowsGateUp && 32 * i < t.ntok ? 32u * i * ldx : 0);
+          __builtin_amdgcn_readfirstlane(MODE != kRowsGateUp && 8 * W * i < t.ntok ? 8u * W * i * ldx : 0);
     if constexpr (MODE == kRowsGateUp) {
 #pragma unroll
       for (int i = 0; i < LB; ++i) {
-        const int tok = a.order[t.r0 + min(row0 + 32 * i, t.ntok - 1)] / a.topk;
-        toff[i] = row0 + 32 * i < t.ntok ? (uint32_t)tok * ldx + tunit : kNowhere;
+        const int tok = a.order[t.r0 + min(row0 + 8 * W * i, t.ntok - 1)] / a.topk;
+        toff[i] = row0 + 8 * W * i < t.ntok ? (uint32_t)tok * ldx + tunit : kNowhere;
       }
     } else {
       toff[0] = row0 * ldx + tunit;
@@ -412,7 +415,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   };
   auto load_a = [&](const Step& st, auto ic) __attribute__((always_inline)) {
     constexpr int i = decltype(ic)::value;
-    dma16_buffer(wbuf, lds + st.stage + (wave + 4 * i) * 1024, woff[i & 1] | st.off[i & 1],
+    dma16_buffer(wbuf, lds + st.stage + (wave + W * i) * 1024, woff[i & 1] | st.off[i & 1],
                  st.k0 + wrow[i]);
   };
   auto load_b = [&](const Step& st, auto ic) __attribute__((always_inline)) {
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
       dma4_buffer(sbuf, lds + st.stage + S::kTRows * 128 + srow * 4, soff | st.off[1],
                   (st.k0 >> 7) * (uint32_t)(a.P * 4));
     else
-      dma16_buffer(xbuf, lds + st.stage + (wave + 4 * i) * 1024,
+      dma16_buffer(xbuf, lds + st.stage + (wave + W * i) * 1024,
                    toff[MODE == kRowsGateUp ? i : 0] | st.off[0], st.k0 + xrow[i]);
   };
   constexpr int NLB = LB + (SC ? 1 : 0);
@@ -555,12 +558,12 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   static_assert(PER >= 4 && 64 % PER == 0 && 16 % (64 / PER) == 0, "whole turns in a token block");
   constexpr int UE = 16 / RPI;  // rows of a lane in a token block
   constexpr int kRow = 16 * NA * 4;
-  static_assert(4 * 16 * kRow == S::kAStage, "the waves' quarters");
+  static_assert(W * 16 * kRow == S::kAStage, "the waves' parts");
   const uint32_t part = lbase + 2 * S::kAStage + wave * 16 * kRow;
   const int c = lane % PER, rsub = lane / PER;
   float ws[8], other[8], xs[NB];  // column scales, and the up scales or the bias; row scales
   auto scales = [&](const Tile& t) __attribute__((always_inline)) {
-    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
+    const int n = t.n0 + wm * (S::kOut / S::kWM) + c * 8;
     if constexpr (MODE == kRowsGateUp) {
       rows_gate_up_cols(a, t.e, n, ws, other);
     } else if constexpr (MODE == kRowsLinear) {
@@ -613,7 +616,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
     return (2 * b + wn) * 16 + rsub + i * RPI;
   };
   auto fetch = [&](const Tile& t, int b, Ops& o) __attribute__((always_inline)) {
-    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
+    const int n = t.n0 + wm * (S::kOut / S::kWM) + c * 8;
 #pragma unroll
     for (int i = 0; i < UE; ++i) {
       const int row = row_of(b, i);
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(256, 1) void k_rows_tile(RowsGemm a, int ncol, int 
   // for the DMA loads, as which it counts the stores here too.
   auto finish = [&](auto with, const Tile& t, int b, int nb, Ops& o) __attribute__((always_inline)) {
     constexpr bool WITH = decltype(with)::value;
-    const int n = t.n0 + wm * (S::kOut / 2) + c * 8;
+    const int n = t.n0 + wm * (S::kOut / S::kWM) + c * 8;
     static_for<NB>([&](auto k) __attribute__((always_inline)) {
       if (b == decltype(k)::value) stage(k);
     });
@@ -886,7 +889,7 @@ hipError_t launch_few(const RowsGemm& a, hipStream_t s) {
 }
 
 // A kernel's dynamic LDS above the default limit, allowed once per device.
-template <int ES, int MODE, int NA, int NB>
+template <int ES, int MODE, int NA, int NB, int W>
 hipError_t allow_tile_lds() {
   static std::mutex mu;
   static uint64_t done = 0;  // bit d: device d
@@ -896,9 +899,9 @@ hipError_t allow_tile_lds() {
   if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(mu);
   if (done >> dev & 1) return hipSuccess;
-  err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_tile<ES, MODE, NA, NB>),
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_tile<ES, MODE, NA, NB, W>),
                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                            TileShape<MODE, NA, NB>::kLds);
+                            TileShape<MODE, NA, NB, W>::kLds);
   if (err == hipSuccess) done |= uint64_t(1) << dev;
   return err;
 }
@@ -917,18 +920,18 @@ int resident(int lds) {
   return n / 8 * 8 * (160 * 1024 / lds);
 }
 
-template <int ES, int MODE, int NA, int NB>
+template <int ES, int MODE, int NA, int NB, int W = 4>
 hipError_t launch_tile(const RowsGemm& a, hipStream_t s) {
-  using S = TileShape<MODE, NA, NB>;
+  using S = TileShape<MODE, NA, NB, W>;
   const long long ncol = (a.N + S::kOut - 1) / S::kOut;
   const long long ntile = MODE == kRowsLinear ? (a.M + S::kTRows - 1) / S::kTRows : a.MT;
   if (ntile <= 0) return hipSuccess;
   const long long tiles = MODE == kRowsLinear ? (ncol * ntile + 7) / 8 * 8 : (ntile + 7) / 8 * 8 * ncol;
   if (tiles > 0x3fffffffLL) return hipErrorInvalidValue;
-  hipError_t err = allow_tile_lds<ES, MODE, NA, NB>();
+  hipError_t err = allow_tile_lds<ES, MODE, NA, NB, W>();
   if (err != hipSuccess) return err;
   const long long grid = std::min<long long>(tiles, resident(S::kLds));
-  hipLaunchKernelGGL((k_rows_tile<ES, MODE, NA, NB>), dim3((unsigned)grid), dim3(256), S::kLds, s, a,
+  hipLaunchKernelGGL((k_rows_tile<ES, MODE, NA, NB, W>), dim3((unsigned)grid), dim3(64 * W), S::kLds, s, a,
                      (int)ncol, (int)ntile);
   return hipGetLastError();
 }
@@ -1023,14 +1026,14 @@ hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_r
     switch (tile_rows) {
       case 64: return launch_tile<1, kRowsGateUp, 4, 2>(a, s);
       case 128: return launch_tile<1, kRowsGateUp, 8, 4>(a, s);
-      case 192: return launch_tile<1, kRowsGateUp, 8, 6>(a, s);
+      case 192: return launch_tile<1, kRowsGateUp, 4, 6, 8>(a, s);
       default: return launch_few<1, kRowsGateUp, 4, 1, 4, 1>(a, s);
     }
   }
   switch (tile_rows) {
     case 64: return launch_tile<1, kRowsDown, 4, 2>(a, s);
     case 128: return launch_tile<1, kRowsDown, 8, 4>(a, s);
-    case 192: return launch_tile<1, kRowsDown, 8, 6>(a, s);
+    case 192: return launch_tile<1, kRowsDown, 4, 6, 8>(a, s);
     default: return launch_few<1, kRowsDown, 2, 1, 4, 1>(a, s);
   }
 }
