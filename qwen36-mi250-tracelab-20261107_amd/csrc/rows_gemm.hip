@@ -38,9 +38,10 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
 }
 
 // Few token rows: 16 NB weight rows times 16 MB token rows a workgroup, K split over its W
-// waves, operands straight from memory into the matrix instructions, the loads of U steps (16 KiB
+// waves, operands straight from memory into the matrix instructions, the loads of U steps (2 NB U KiB
 // of weights a wave) together; the waves' sums meet in LDS in a fixed order. Bound by the stream of
-// weights, for one token by its latency.
+// weights (32 tokens of 256 experts, H = 2048, I = 512: gate_up 5.0 TB/s, down 4.9), for one token
+// by its latency (2048 x 2048 bf16 5.4 us).
 template <int ES, int MODE, int NB, int MB, int W, int U>
 __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   __shared__ f32x4_t red[W][NB * MB][64];
@@ -175,10 +176,14 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   }
 }
 
-// Many token rows: 32 NA weight rows times 32 NB token rows a workgroup of four waves, both operands
-// staged in LDS. Wave (wm, wn) owns 16 NA weight rows and every other 16-row token block: 16 x 16
-// blocks acc[NA][NB], so each fragment read from LDS feeds NA or NB matrix instructions (at NA = NB = 8
-// the reads of a step take half the time of its products; with 64 x 128 blocks, three quarters).
+// Many token rows: 16 NA kWM weight rows times 32 NB token rows a workgroup of W = 2 kWM waves, both
+// operands staged in LDS. Wave (wm, wn) owns 16 NA weight rows and every other 16-row token block:
+// 16 x 16 blocks acc[NA][NB], so each fragment read from LDS feeds NA or NB matrix instructions (at NA =
+// NB = 8 the reads of a step take half the time of its products; with 64 x 128 blocks, three quarters).
+// Linear: four waves, a SIMD's whole register file each, since the products are the bound (8192^2, K =
+// 2048 bf16 270 us, 273 with eight waves; K = 4096 e4m3 220 and 229). The experts' larger tiles wait for
+// memory and take long in their epilogue: eight waves, which wait in turns (4096 tokens as below 299 ->
+// 276 us).
 //
 // Staging. A step of K (128 bytes of a row) is loaded memory -> LDS by DMA, eight rows (1 KiB) a load
 // of a wave, into rings of SA weight and SB token stages: step d + SA of the weights and d + SB of the
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
     rb[0] = rb[1], rb[1] = u0;
   };
 
-  // ---- epilogue: a token block (16 rows) of a wave at a time through its quarter of a weight stage, so that
+  // ---- epilogue: a token block (16 rows) of a wave at a time through its part of a weight stage, so that
   // one small loop serves all of the sums (unrolled over the registers it was 80 KB of instructions,
   // which took longer to fetch than a tile of K = 1024 to multiply) and a row's outputs are stored
   // together. Unit u of row r lies at unit u ^ (r & 7), so that eight rows differ in banks.
@@ -979,10 +984,11 @@ hipError_t launch_linear(const RowsGemm& a, hipStream_t s) {
 // Up to 16 pairs, or one for every four experts, no tiles: few share an expert, and there is nothing to
 // sort (us, H = 2048, I = 512, 256 experts, each pair by itself / tiles of 16: 32 pairs 25, 34; 64 41,
 // 50; 128 75, 74; 16 experts of H = 4096, I = 1024: 32 pairs 79, 48). Else by the pairs r of an expert on
-// average (256 experts as above, tiles of 16 / 64 / 128 / 192 pairs: r = 4 162, 168, 186, 199; r = 16 253, 185, 207, 218; r = 32 398, 194,
-// 210, 225; r = 64 667, 251, 230, 246; r = 128 1185, 387, 325, 295). Tiles of 128 and 192 take a CU each
-// and 128 outputs of gate_up: where these are too few workgroups, 64 (8 experts, r = 256: 46 us, 56 with
-// 192; 16 experts of H = 4096, I = 1024, r = 128: 128 workgroups, 105 and 88).
+// average (256 experts as above, tiles of 16 / 64 / 128 / 192 pairs: r = 4 162, 172, 182, 191; r = 16 252,
+// 191, 199, 208; r = 32 396, 201, 202, 214; r = 64 668, 253, 225, 240; r = 128 1187, 391, 307, 277). Tiles
+// of 128 and 192 take a CU each and 128 outputs of gate_up: where these are under half a chip of
+// workgroups, the next smaller tile (8 experts, r = 512: 70, 62 with 128, 59 with 192 for 96 workgroups;
+// r = 256: 48, 47, 52).
 int rows_tile_rows(int T, int H, int E, int k, int I) {
   const long long P = (long long)T * k;
   if (P <= std::max(16, E / 4)) return 0;
@@ -994,8 +1000,8 @@ int rows_tile_rows(int T, int H, int E, int k, int I) {
     return (P + E * rows - 1) / (E * rows) * E * ((I + 127) / 128);
   };
   if (P <= 48LL * E) return 64;
-  const int rows = P <= 96LL * E ? 128 : 192;
-  return workgroups(rows) >= 128 ? rows : 64;
+  if (P > 96LL * E && workgroups(192) >= 128) return 192;
+  return workgroups(128) >= 128 ? 128 : 64;
 }
 
 hipError_t launch_rows_pairs_down(const RowsGemm& a, const RowsTail& tail, int T, hipStream_t s) {
@@ -1025,14 +1031,14 @@ hipError_t launch_rows_gemm(RowsMode mode, int es, const RowsGemm& a, int tile_r
   if (mode == kRowsGateUp) {
     switch (tile_rows) {
       case 64: return launch_tile<1, kRowsGateUp, 4, 2>(a, s);
-      case 128: return launch_tile<1, kRowsGateUp, 8, 4>(a, s);
+      case 128: return launch_tile<1, kRowsGateUp, 4, 4, 8>(a, s);
       case 192: return launch_tile<1, kRowsGateUp, 4, 6, 8>(a, s);
       default: return launch_few<1, kRowsGateUp, 4, 1, 4, 1>(a, s);
     }
   }
   switch (tile_rows) {
     case 64: return launch_tile<1, kRowsDown, 4, 2>(a, s);
-    case 128: return launch_tile<1, kRowsDown, 8, 4>(a, s);
+    case 128: return launch_tile<1, kRowsDown, 4, 4, 8>(a, s);
     case 192: return launch_tile<1, kRowsDown, 4, 6, 8>(a, s);
     default: return launch_few<1, kRowsDown, 2, 1, 4, 1>(a, s);
   }
