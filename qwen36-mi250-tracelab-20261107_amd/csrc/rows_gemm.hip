@@ -207,7 +207,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // take 2048.)
 //
 // A workgroup walks over tiles, as many workgroups as the chip holds. The next tile's first two steps
-// are requested before the present one's epilogue, which needs only the third weight stage of LDS, so
+// are requested before the present one's epilogue, which needs only the last weight stage of LDS, so
 // that memory is not idle meanwhile.
 struct Frag {
   u32x4v v[2];
@@ -282,7 +282,10 @@ template <int MODE, int NA, int NB, int W>
 struct TileShape {
   static constexpr int kWM = W / 2;  // waves side by side along the weight rows
   static constexpr int kWRows = 16 * NA * kWM, kTRows = 32 * NB;
-  static constexpr int kSA = 3, kSB = 2;
+  // Small tiles, whose fragments of a step fit in registers twice. Stages: as many as leave two workgroups
+  // a CU.
+  static constexpr bool kFlat = W == 4 && NA * NB <= 8;
+  static constexpr int kSA = kFlat && NA == 2 ? 4 : 3, kSB = kFlat ? kSA : 2;
   static constexpr bool kScaled = MODE == kRowsDown;
   static constexpr int kAStage = kWRows * 128;
   static constexpr int kBStage = kTRows * 128 + (kScaled ? kTRows * 4 : 0);
@@ -295,7 +298,7 @@ struct TileShape {
 template <int ES, int MODE, int NA, int NB, int W>
 __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, int ntile) {
   using S = TileShape<MODE, NA, NB, W>;
-  constexpr bool SC = S::kScaled;
+  constexpr bool SC = S::kScaled, FLAT = S::kFlat;
   constexpr int HA = NA / 2, HB = NB / 2;
   constexpr int LA = S::kWRows / (8 * W), LB = S::kTRows / (8 * W);  // loads of a wave and step
   extern __shared__ uint4 smem[];
@@ -434,13 +437,22 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   };
   constexpr int NLB = LB + (SC ? 1 : 0);
   constexpr int kB0 = S::kSA * S::kAStage;  // the token ring
-  // The first two steps' loads, in the order in which the steps issue them: tokens, then weights one
-  // further on (the third weights, whose stage the epilogue uses, are requested at the tile's start)
+  // The first steps' loads, in the order in which the steps issue them: tokens, then weights one
+  // further on (what goes to the last weight stage, which the epilogue uses, is requested at the tile's start)
   auto first_loads = [&]() __attribute__((always_inline)) {
-    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(0, 0), k); });
-    static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(0, kB0), k); });
-    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(1, S::kAStage), k); });
-    static_for<NLB>([&](auto k) __attribute__((always_inline)) { load_b(step_b(1, kB0 + S::kBStage), k); });
+    static_for<S::kSA - 1>([&](auto dc) __attribute__((always_inline)) {
+      constexpr int d = decltype(dc)::value;
+      static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(d, d * S::kAStage), k); });
+      static_for<NLB>([&](auto k)
+                          __attribute__((always_inline)) { load_b(step_b(d, kB0 + d * S::kBStage), k); });
+    });
+  };
+  auto last_loads = [&]() __attribute__((always_inline)) {
+    constexpr int d = S::kSA - 1;
+    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(d, d * S::kAStage), k); });
+    if constexpr (FLAT)
+      static_for<NLB>([&](auto k)
+                          __attribute__((always_inline)) { load_b(step_b(d, kB0 + d * S::kBStage), k); });
   };
 
   // ---- fragments
@@ -468,15 +480,16 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   };
 
   f32x4_t acc[NA][NB];
-  Frag a0[HA], a1[HA], bx[HB], by[HB];
-  uint32_t sx[HB] = {}, sy[HB] = {};
-  auto ready_a = [&](Frag (&f)[HA]) __attribute__((always_inline)) {
+  constexpr int FA = FLAT ? NA : HA, FB = FLAT ? NB : HB;
+  Frag a0[FA], a1[FA], bx[FB], by[FB];
+  uint32_t sx[FB] = {}, sy[FB] = {};
+  auto ready_a = [&](Frag (&f)[FA]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < HA; ++i) after_wait(f[i].v[0]), after_wait(f[i].v[1]);
+    for (int i = 0; i < FA; ++i) after_wait(f[i].v[0]), after_wait(f[i].v[1]);
   };
-  auto ready_b = [&](Frag (&f)[HB], uint32_t (&sc)[HB]) __attribute__((always_inline)) {
+  auto ready_b = [&](Frag (&f)[FB], uint32_t (&sc)[FB]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < HB; ++i) {
+    for (int i = 0; i < FB; ++i) {
       after_wait(f[i].v[0]), after_wait(f[i].v[1]);
       if (SC) {
         asm volatile("" : "+v"(sc[i]));
@@ -489,7 +502,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   // second ones, so that no product waits for the one before), what falls due: read k of NR at
   // product RS k, load k of NL at product (k PROD) / NL (one later where there is room).
   constexpr int PROD = HA * HB * ES;
-  auto quarter = [&](const Frag (&w)[HA], const Frag (&tk)[HB], const uint32_t (&sc)[HB], auto xh, auto yh,
+  auto quarter = [&](const Frag (&w)[FA], const Frag (&tk)[FB], const uint32_t (&sc)[FB], auto xh, auto yh,
                      auto nr, auto read, auto nl, auto load) __attribute__((always_inline)) {
     constexpr int X = decltype(xh)::value, Y = decltype(yh)::value;
     constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value;
@@ -516,9 +529,16 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   const integral_constant<int, HB> chb{};
   const auto none = [](auto) {};
   // Ring offsets: the stages of this step and the next ones.
-  uint32_t ra[3], rb[2];
+  uint32_t ra[S::kSA], rb[S::kSB];
+  auto turn = [](auto& r) __attribute__((always_inline)) {
+    constexpr int n = sizeof(r) / sizeof(r[0]);
+    const uint32_t first = r[0];
+#pragma unroll
+    for (int i = 0; i + 1 < n; ++i) r[i] = r[i + 1];
+    r[n - 1] = first;
+  };
   // Step d with its tokens' half 0 in p; half 1 goes to q, and the next step's half 0 after it.
-  auto step = [&](int d, Frag (&p)[HB], uint32_t (&sp)[HB], Frag (&q)[HB], uint32_t (&sq)[HB])
+  auto step = [&](int d, Frag (&p)[FB], uint32_t (&sp)[FB], Frag (&q)[FB], uint32_t (&sq)[FB])
                   __attribute__((always_inline)) {
     const uint32_t at = aaddr + ra[0], at1 = aaddr + ra[1];
     quarter(a0, p, sp, c0, c0, chb, [&](auto k) __attribute__((always_inline)) {
@@ -529,11 +549,11 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
     ready_b(q, sq);
     wait_loads(LA + NLB);  // in flight: step d + 1's tokens, step d + 2's weights
     __builtin_amdgcn_s_barrier();
-    const Step nb2 = step_b(d + 2, rb[0]), na3 = step_a(d + 3, ra[0]);
+    const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
     quarter(a0, q, sq, c0, c1, cha, [&](auto k) __attribute__((always_inline)) {
       constexpr int K = decltype(k)::value;
       read_a(at, integral_constant<int, HA + K>{}, a1[K]);
-    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb2, k); });
+    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb, k); });
     lds_frags_ready();
     ready_a(a1);
     quarter(a1, q, sq, c1, c1, cha, [&](auto k) __attribute__((always_inline)) {
@@ -546,12 +566,52 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
     quarter(a1, p, sp, c1, c0, chb, [&](auto k) __attribute__((always_inline)) {
       constexpr int K = decltype(k)::value;
       read_b(rb[1], k, q[K], sq[K]);
-    }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na3, k); });
+    }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na, k); });
     lds_frags_ready();
     ready_b(q, sq);
-    const uint32_t t0 = ra[0], u0 = rb[0];
-    ra[0] = ra[1], ra[1] = ra[2], ra[2] = t0;
-    rb[0] = rb[1], rb[1] = u0;
+    turn(ra), turn(rb);
+  };
+
+  // A small tile's step: its fragments are in registers (w, tk), the next step's are read to others
+  // during its products, and what is a ring's length on is loaded to the stages that it was read from.
+  // One barrier and one wait for LDS; in quarters there are four, with a product or two between them
+  // (64 x 2048 x 2048 bf16 11.2 us in quarters, 9.6 so; 128 x 64 blocks a wave and larger hide theirs).
+  auto flat_step = [&](int d, const Frag (&w)[FA], const Frag (&tk)[FB], const uint32_t (&sc)[FB],
+                       Frag (&wn)[FA], Frag (&tn)[FB], uint32_t (&sn)[FB])
+                       __attribute__((always_inline)) {
+    wait_loads((S::kSA - 2) * (LA + NLB));  // step d + 1 has arrived
+    __builtin_amdgcn_s_barrier();
+    const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
+    const uint32_t at = aaddr + ra[1];
+    constexpr int ALL = NA * NB * ES, NL = LA + NLB;
+    static_for<ALL>([&](auto prod) __attribute__((always_inline)) {
+      constexpr int p = decltype(prod)::value, H = p / (NA * NB), i = p / NA % NB, j = p % NA;
+      tile_mma<ES, SC, H>(w[j], tk[i], sc[i], acc[j][i]);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<NA + NB>([&](auto kc) __attribute__((always_inline)) {
+        constexpr int k = decltype(kc)::value;
+        if constexpr ((k < ALL ? k : ALL - 1) == p) {
+          if constexpr (k < NB)
+            read_b(rb[1], kc, tn[k], sn[k]);
+          else
+            read_a(at, integral_constant<int, k - NB>{}, wn[k - NB]);
+        }
+      });
+      static_for<NL>([&](auto kc) __attribute__((always_inline)) {
+        constexpr int k = decltype(kc)::value;
+        if constexpr (k * ALL / NL == p) {
+          if constexpr (k < LA)
+            load_a(na, kc);
+          else
+            load_b(nb, integral_constant<int, k - LA>{});
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    lds_frags_ready();
+    ready_a(wn);
+    ready_b(tn, sn);
+    turn(ra), turn(rb);
   };
 
   // ---- epilogue: a token block (16 rows) of a wave at a time through its part of a weight stage, so that
@@ -564,7 +624,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   constexpr int UE = 16 / RPI;  // rows of a lane in a token block
   constexpr int kRow = 16 * NA * 4;
   static_assert(W * 16 * kRow == S::kAStage, "the waves' parts");
-  const uint32_t part = lbase + 2 * S::kAStage + wave * 16 * kRow;
+  const uint32_t part = lbase + (S::kSA - 1) * S::kAStage + wave * 16 * kRow;
   const int c = lane % PER, rsub = lane / PER;
   float ws[8], other[8], xs[NB];  // column scales, and the up scales or the bias; row scales
   auto scales = [&](const Tile& t) __attribute__((always_inline)) {
@@ -696,17 +756,19 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   set_sources(cur);
   first_loads();
   for (;;) {
-    static_for<LA>([&](auto k) __attribute__((always_inline)) { load_a(step_a(2, 2 * S::kAStage), k); });
-    ra[0] = 0, ra[1] = S::kAStage, ra[2] = 2 * S::kAStage;
-    rb[0] = kB0, rb[1] = kB0 + S::kBStage;
+    last_loads();
+#pragma unroll
+    for (int i = 0; i < S::kSA; ++i) ra[i] = i * S::kAStage;
+#pragma unroll
+    for (int i = 0; i < S::kSB; ++i) rb[i] = kB0 + i * S::kBStage;
 #pragma unroll
     for (int x = 0; x < NA; ++x)
 #pragma unroll
       for (int y = 0; y < NB; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    wait_loads(2 * LA + NLB);  // step 0 has arrived
+    wait_loads((S::kSB - 1) * (LA + NLB) + (FLAT ? 0 : LA));  // step 0 has arrived
     __builtin_amdgcn_s_barrier();
-    static_for<HA>([&](auto k) __attribute__((always_inline)) { read_a(aaddr, k, a0[decltype(k)::value]); });
-    static_for<HB>([&](auto k) __attribute__((always_inline)) {
+    static_for<FA>([&](auto k) __attribute__((always_inline)) { read_a(aaddr, k, a0[decltype(k)::value]); });
+    static_for<FB>([&](auto k) __attribute__((always_inline)) {
       constexpr int K = decltype(k)::value;
       read_b(kB0, k, bx[K], sx[K]);
     });
@@ -714,8 +776,13 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
     ready_a(a0);
     ready_b(bx, sx);
     for (int d = 0; d < nd; d += 2) {
-      step(d, bx, sx, by, sy);
-      step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
+      if constexpr (FLAT) {
+        flat_step(d, a0, bx, sx, a1, by, sy);
+        flat_step(d + 1, a1, by, sy, a0, bx, sx);
+      } else {
+        step(d, bx, sx, by, sy);
+        step(d + 1, by, sy, bx, sx);  // of zeros if nd is odd
+      }
     }
     wait_loads(0);
     mma_done(acc);
@@ -759,7 +826,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
       for (int b = 0; b < nb; ++b) finish(std::false_type{}, cur, b, nb, s0);
     }
     if (!more) return;
-    __builtin_amdgcn_s_barrier();  // the third weight stage is free
+    __builtin_amdgcn_s_barrier();  // the last weight stage is free
     cur = next;
   }
 }
