@@ -192,7 +192,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // last one and bytes past a row's end lie outside the load's buffer and come as zeros.
 //
 // Order of the weight rows: row 4 q + i of block b is the wave's output 4 NA q + 4 b + i, so a lane
-// ends with 4 NA neighbouring outputs (2 NA gate and 2 NA up ones, half a group of 32) of each token
+// ends with 4 NA neighbouring outputs (or 2 NA gate and 2 NA up ones) of each token
 // and stores them in 16-byte pieces.
 //
 // A step's products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0). Between
