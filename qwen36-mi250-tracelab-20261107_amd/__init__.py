@@ -8,7 +8,9 @@ include/moe_mi355x.h):
   implementation (engine/experts.py:93-108).
 - ``block.moe(x, mlp, top_k)``: the whole block, router to combine
   (engine/fast/model.py:1139, engine/fast/prefill_kernels.py:676).
-- ``ops``: the individual operations (route, sort, grouped GEMMs, combine).
+- ``block.add_rms_moe_fp8``: a layer's add + RMSNorm and block with 8-bit activations.
+- ``ops``: the individual operations (route, sort, grouped GEMMs, combine; 8-bit rows, the fused
+  linear and the experts on 8-bit rows).
 - ``fp8``: per-row fp8-e4m3 expert weights; ``checkpoint``: their on-disk format (quantise a
   bf16 safetensors snapshot once, load the fp8 layers).
 - ``graphs.MoeGraphs``: the block captured once per decode bucket and replayed.
