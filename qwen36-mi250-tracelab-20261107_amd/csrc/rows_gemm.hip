@@ -108,7 +108,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
     int sv[U][MB];
 #pragma unroll
     for (int s = 0; s < U; ++s) {
-      // past the wave's part or the row's end: bytes there again, the token's as zeros
+      // past the wave's part or the row's end: bytes there again, below made zeros
       const int k0 = (c + s) * 128 + kq * 16, k1 = k0 + 64;
       const int o0 = min(k0, a.Kb - 16), o1 = min(k1, a.Kb - 16);
 #pragma unroll
@@ -131,6 +131,13 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
       for (int m = 0; m < MB; ++m) {
         if (k0 >= end) xv[s][m][0] = make_uint4(0u, 0u, 0u, 0u);
         if (k1 >= end) xv[s][m][1] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (ES == 2) {  // whose weights may be infinite, and zero times that is NaN
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          if (k0 >= end) wv[s][b][0] = make_uint4(0u, 0u, 0u, 0u);
+          if (k1 >= end) wv[s][b][1] = make_uint4(0u, 0u, 0u, 0u);
+        }
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b)

@@ -199,3 +199,20 @@ def test_linear_refusals(pkg, dev):
                 lambda: lin(x, w, bias=torch.zeros(6))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("M,K", [(1, 40), (20, 200), (70, 72), (300, 2056)])
+def test_linear_infinite_weights_and_rows_stay_infinite(pkg, dev, M, K):
+    """An infinity in the last columns, beside bytes past a row's end, is no NaN: positive rows times a
+    weight of plus and one of minus infinity, and the other way round."""
+    g = torch.Generator().manual_seed(K)
+    x, w = (torch.rand(M, K, generator=g) + 0.5).to(BF16), (torch.rand(40, K, generator=g) + 0.5).to(BF16)
+    w[3, K - 1], w[5, K - 8], w[39, 0] = torch.inf, -torch.inf, torch.inf
+    got = pkg.ops.linear(x.to(dev), w.to(dev)).float().cpu()
+    for n, sign in ((3, 1), (5, -1), (39, 1)):
+        assert (got[:, n] == sign * torch.inf).all(), n
+    rest = [n for n in range(40) if n not in (3, 5, 39)]
+    assert torch.isfinite(got[:, rest]).all()
+    x[0, K - 1] = -torch.inf
+    got = pkg.ops.linear(x.to(dev), w.to(dev)).float().cpu()
+    assert (got[0, rest] == -torch.inf).all() and torch.isfinite(got[1:, rest]).all()
