@@ -134,7 +134,8 @@ __device__ __forceinline__ void rows_act(float (&v)[C], int act) {
     const float c0 = act == kActSilu ? 1.0f : 1.5957691216057308f;
     const float c1 = act == kActSilu ? 0.0f : 1.5957691216057308f * 0.044715f;
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = rows_gate(v[i], v[i] * fmaf(c1, v[i] * v[i], c0));
+    for (int i = 0; i < C; ++i)  // the square may overflow, and 0 inf is NaN
+      v[i] = rows_gate(v[i], v[i] * fmaf(c1, fminf(v[i] * v[i], 1e30f), c0));
   } else if (act == kActRelu) {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN

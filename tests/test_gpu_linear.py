@@ -216,3 +216,16 @@ def test_linear_infinite_weights_and_rows_stay_infinite(pkg, dev, M, K):
     x[0, K - 1] = -torch.inf
     got = pkg.ops.linear(x.to(dev), w.to(dev)).float().cpu()
     assert (got[0, rest] == -torch.inf).all() and torch.isfinite(got[1:, rest]).all()
+
+
+def test_linear_activations_of_huge_values(pkg, dev):
+    """Values whose square leaves fp32, and infinity: the identity above zero, zero below (bf16 of a finite
+    value up to its largest is itself)."""
+    v = torch.tensor([1e19, 1e20, 3e38, 1e30], dtype=BF16)
+    x, w = torch.zeros(1, 16, dtype=BF16), torch.zeros(8, 16, dtype=BF16)
+    for act in ACTS[1:]:
+        got = pkg.ops.linear(x.to(dev), w.to(dev), bias=torch.cat([v, -v]).to(dev), activation=act)[0].cpu()
+        assert torch.equal(got[:4], v), act
+        assert (got[4:] == 0).all(), act
+        inf = torch.full((8,), torch.inf, dtype=BF16, device=dev)
+        assert (pkg.ops.linear(x.to(dev), w.to(dev), bias=inf, activation=act) == torch.inf).all(), act
