@@ -945,7 +945,6 @@ bool overlaps(const void* a, const void* b, size_t bytes) {
   return a && b && p < q + bytes && q < p + bytes;
 }
 
-// The aliasing and alignment rules of the add + RMSNorm entry points.
 // The bytes an argument covers (p null: none), and whether outputs keep clear of the inputs and of
 // each other.
 struct Span {
@@ -995,6 +994,7 @@ Experts8Ws carve_experts8(void* base, int T, int H, int E, int k, int I) {
   return w;
 }
 
+// The aliasing and alignment rules of the add + RMSNorm entry points.
 int check_norm_args(const void* x, const void* h, const void* w, int T, int H, float eps,
                     const void* total, const void* norm, const void* out) {
   CHECK_ARG(T >= 0 && H > 0 && H % 8 == 0 && H <= 512 * kAddRmsMaxChunks,
@@ -1174,7 +1174,9 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
   CHECK_ARG(dtype == MOE_WEIGHTS_BF16 || dtype == MOE_WEIGHTS_FP8_E4M3, "linear: bad dtype %d",
             dtype);
   const int es = dtype == MOE_WEIGHTS_BF16 ? 2 : 1;
-  CHECK_ARG(M >= 0 && N >= 0, "linear: M and N must be >= 0 (got %d, %d)", M, N);
+  constexpr int kMost = 0x7fffffff - 1024;  // the kernels round up to whole tiles
+  CHECK_ARG(M >= 0 && N >= 0 && M <= kMost && N <= kMost,
+            "linear: M and N must be >= 0 and at most %d (got %d, %d)", kMost, M, N);
   CHECK_ARG(K >= 16 / es && K % (16 / es) == 0 && K <= (1 << 28),
             "linear: K must be a positive multiple of %d (got %d)", 16 / es, K);
   CHECK_ARG(act >= MOE_ACT_NONE && act <= MOE_ACT_GELU_TANH, "linear: bad activation %d", act);
@@ -1230,13 +1232,16 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
   CHECK_ARG(((uintptr_t)q | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)shared |
              (uintptr_t)residual | (uintptr_t)out | (uintptr_t)workspace) % 16 == 0,
             "experts_fp8: q, the weights, shared, residual, out and the workspace must be 16-byte aligned");
-  const long long row = 2LL * T * H;
-  const Span in[] = {{q, row / 2}, {shared, row}, {residual, row}};
-  const Span o{out, row};
-  CHECK_ARG(apart(in, 3, &o, 1), "experts_fp8: out must not overlap the inputs");
   const Experts8Ws w = carve_experts8(workspace, T, H, E, k, I);
   CHECK_ARG(workspace && workspace_bytes >= w.bytes, "experts_fp8: workspace too small: %zu < %zu",
             workspace_bytes, w.bytes);
+  const long long row = 2LL * T * H, pairs = (long long)T * k, proj = (long long)E * H * I;
+  const Span in[] = {{q, row / 2}, {x_scale, 4LL * T}, {top_k_index, 8 * pairs},
+                     {top_k_weights, 2 * pairs}, {gate_up, 2 * proj}, {gu_scale, 8LL * E * I},
+                     {down, proj}, {dn_scale, 4LL * E * H}, {shared, row}, {residual, row}};
+  const Span o[] = {{out, row}, {workspace, (long long)w.bytes}};
+  CHECK_ARG(apart(in, 10, o, 2),
+            "experts_fp8: out and the workspace must not overlap the inputs or each other");
   hipStream_t s = (hipStream_t)stream;
   const uint16_t* wts = static_cast<const uint16_t*>(top_k_weights);
   const RowsTail tail{static_cast<const uint16_t*>(shared),

@@ -72,6 +72,8 @@ def test_linear_refusals(pkg):
     _refused(pkg, call(bias=D + 2, f32=1), b"aligned")
     _refused(pkg, call(out=A), b"overlap")
     _refused(pkg, call(res=C + 8), b"overlap")
+    _refused(pkg, call(N=2**31 - 1), b"M and N")
+    _refused(pkg, call(M=2**31 - 512), b"M and N")
     assert call(M=0, x=None) == 0 and call(N=0, w=None) == 0
 
 
@@ -103,6 +105,9 @@ def test_experts_fp8_refusals(pkg):
     _refused(pkg, call(res=B + 8), b"aligned")
     _refused(pkg, call(res=C), b"overlap")
     _refused(pkg, call(sh=C + 64, gate=B), b"overlap")
+    for name in ("q", "gu", "dn"):
+        _refused(pkg, call(**{name: D + 64}), b"overlap")
+    _refused(pkg, call(out=D + 128), b"overlap")
     assert call(T=0, q=None) == 0
 
 
