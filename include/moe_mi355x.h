@@ -242,7 +242,8 @@ int moe_block_forward_add_rms(const void* x, const void* h, const void* norm_wei
  * 2^-100 at least; 1 for a row of zeros), values e4m3(v / s), ties to even; NaN and infinite
  * values become NaN. */
 
-/* q [T, n] e4m3 and scale [T] fp32 of x [T, n] bf16; n a multiple of 8 up to 8192. */
+/* q [T, n] e4m3 and scale [T] fp32 of x [T, n] bf16; n a multiple of 8 up to 8192, T at
+ * most 2^26 - 4 (here and below). */
 int moe_quantize_rows(const void* x, int T, int n, void* q, float* scale, void* stream);
 
 /* moe_add_rmsnorm with the norm in 8 bits, made from its fp32 values: q [T, H], scale [T], and

@@ -14,6 +14,7 @@
 namespace moe {
 
 constexpr float kE4m3Max = 448.0f;
+constexpr int kMostRows = (1 << 26) - 4;  // a launch has fewer than 2^32 threads, 64 a row
 
 __device__ __forceinline__ float row_scale(float amax) {
   return amax > 0.f ? fmaxf(amax, 0x1p-100f) / kE4m3Max : 1.0f;

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void k_add_rms_fp8(const uint16_t* x, const ui
 hipError_t launch_quantize_rows(const uint16_t* x, int T, int n, uint8_t* q, float* scale,
                                 hipStream_t s) {
   if (T <= 0) return hipSuccess;
-  if (n <= 0 || n % 8 || n > 512 * kAddRmsMaxChunks) return hipErrorInvalidValue;
+  if (n <= 0 || n % 8 || n > 512 * kAddRmsMaxChunks || T > kMostRows) return hipErrorInvalidValue;
   const dim3 grid((T + 3) / 4), block(256);
   const int hc = (n + 511) / 512;
 #define L(HC)                                                                      \
@@ -126,7 +126,7 @@ hipError_t launch_add_rms_fp8(const uint16_t* x, const uint16_t* h, const uint16
                               float eps, uint16_t* total, uint8_t* q, float* scale, uint16_t* norm,
                               hipStream_t s) {
   if (T <= 0) return hipSuccess;
-  if (H <= 0 || H % 8 || H > 512 * kAddRmsMaxChunks) return hipErrorInvalidValue;
+  if (H <= 0 || H % 8 || H > 512 * kAddRmsMaxChunks || T > kMostRows) return hipErrorInvalidValue;
   const dim3 grid((T + 3) / 4), block(256);
   const int hc = (H + 511) / 512;
 #define L(HC)                                                                                \

@@ -1132,6 +1132,7 @@ int moe_quantize_rows(const void* x, int T, int n, void* q, float* scale, void* 
   CHECK_ARG(T >= 0 && n > 0 && n % 8 == 0 && n <= 512 * kAddRmsMaxChunks,
             "quantize_rows: rows must be a positive multiple of 8 up to %d long (got %d)",
             512 * kAddRmsMaxChunks, n);
+  CHECK_ARG(T <= kMostRows, "quantize_rows: at most %d rows (got %d)", kMostRows, T);
   if (T == 0) return MOE_OK;
   CHECK_ARG(x && q && scale, "quantize_rows: null pointer");
   CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)q % 8 == 0 && (uintptr_t)scale % 4 == 0,
@@ -1148,6 +1149,7 @@ int moe_add_rmsnorm_fp8(const void* x, const void* h, const void* weight, int T,
   CHECK_ARG(T >= 0 && H > 0 && H % 8 == 0 && H <= 512 * kAddRmsMaxChunks,
             "add_rms_fp8: H must be a positive multiple of 8 up to %d (got %d)",
             512 * kAddRmsMaxChunks, H);
+  CHECK_ARG(T <= kMostRows, "add_rms_fp8: at most %d rows (got %d)", kMostRows, T);
   CHECK_ARG(eps >= 0.f, "add_rms_fp8: eps must be >= 0 (got %g)", (double)eps);
   if (T == 0) return MOE_OK;
   CHECK_ARG(x && weight && q && scale && (!h || total), "add_rms_fp8: null pointer");

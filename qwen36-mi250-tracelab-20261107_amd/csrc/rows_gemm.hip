@@ -953,7 +953,7 @@ hipError_t launch_few(const RowsGemm& a, hipStream_t s) {
   const long long tiles = MODE == kRowsLinear     ? (a.M + 16 * MB - 1) / (16 * MB)
                           : a.ids && !a.table ? a.P
                                               : a.MT;
-  if (cols > 0x7fffffffLL || tiles > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (cols * W * 64 > 0xffffffffLL || tiles > 0x7fffffffLL) return hipErrorInvalidValue;
   constexpr long long kGridY = 65535;
   for (long long i = 0; i < tiles; i += kGridY) {
     RowsGemm part = a;
@@ -1090,7 +1090,7 @@ hipError_t launch_rows_combine(const uint16_t* y, const uint8_t* yexp, const uin
                                hipStream_t s) {
   if (T <= 0) return hipSuccess;
   const long long grid = ((long long)T * (H / 8) + 255) / 256;
-  if (H % 32 || grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (H % 32 || grid * 256 > 0xffffffffLL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)grid), dim3(256), 0, s, y, yexp, w, tail, T, H, k,
                      out);
   return hipGetLastError();

@@ -456,6 +456,12 @@ def _call(name: str, dev: int, fn, *args) -> None:
         check(rc, name)
 
 
+def _sizes(name: str, *sizes: int) -> None:
+    """The C entry points take ints, to which ctypes would cut larger sizes."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{name}: sizes must be below 2^31 (got {max(sizes)})")
+
+
 _F32 = (torch.float32,)
 _BIAS = (torch.bfloat16, torch.float32)
 
@@ -466,9 +472,10 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     as 2^-100 at least) and q = e4m3(x / scale), ties to even. NaN and infinite values become NaN.
     The format of ``fp8.quantize_rows``, for activations."""
     x = _input(x, torch.bfloat16, "x")
-    n, dev = x.shape[-1], x.get_device()
+    n, dev = x.shape[-1] if x.dim() else 0, x.get_device()
     q = torch.empty_like(x, dtype=FP8)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _sizes("quantize_rows", scale.numel(), n)
     _call("quantize_rows", dev, _lib.load().moe_quantize_rows, x.data_ptr(), scale.numel(), n,
           q.data_ptr(), scale.data_ptr())
     return q, scale
@@ -481,7 +488,7 @@ def add_rms_fp8(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, e
     the fp32 norm: it is rounded once, not to bf16 first. With ``h`` None total is ``x``."""
     x = _input(x, torch.bfloat16, "x")
     shape, dev = x.shape, x.get_device()
-    n = shape[-1]
+    n = shape[-1] if shape else 0
     weight = _input(weight, torch.bfloat16, "weight", dev)
     if weight.numel() != n:
         raise ValueError(f"weight must have {n} elements (got {weight.numel()})")
@@ -495,6 +502,7 @@ def add_rms_fp8(x: torch.Tensor, h: torch.Tensor | None, weight: torch.Tensor, e
     q = torch.empty_like(x, dtype=FP8)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
     norm = torch.empty_like(x) if return_norm else None
+    _sizes("add_rms_fp8", scale.numel(), n)
     _call("add_rms_fp8", dev, _lib.load().moe_add_rmsnorm_fp8, x.data_ptr(), ptr(h),
           weight.data_ptr(), scale.numel(), n, eps, added, q.data_ptr(), scale.data_ptr(), ptr(norm))
     return (total, q, scale, norm) if return_norm else (total, q, scale)
@@ -520,7 +528,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
     if w.dtype is not kind or not (kind is torch.bfloat16 or kind is FP8):
         raise ValueError(f"x and w must both be bfloat16 or float8_e4m3fn (got {kind}, {w.dtype})")
     shape, dev = x.shape, x.get_device()
-    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1]:
+    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1] or not shape[-1]:
         raise ValueError(f"x {tuple(shape)} and w {tuple(w.shape)} do not match")
     if w.get_device() != dev:
         raise ValueError(f"w is on {w.device}, x on {x.device}")
@@ -538,6 +546,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
         w_scale = _vector(w_scale, _F32, "w_scale", n, dev).data_ptr()
     elif x_scale is not None or w_scale is not None:
         raise ValueError("bf16 operands take no scales")
+    _sizes("linear", rows, n, k)
     out_shape = (*shape[:-1], n)
     bias_f32 = 0
     if bias is not None:
@@ -605,6 +614,7 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
         if t.get_device() != dev:
             raise ValueError(f"{name} is on {t.device}, q on {q.device}")
     top_k = top_k_index.shape[1]
+    _sizes("experts_fp8", tokens, hidden, nexp, two_i)
     scale = _vector(scale, _F32, "scale", tokens, dev)
     gus = _vector(gate_up_scale, _F32, "gate_up_scale", nexp * two_i, dev)
     dns = _vector(down_scale, _F32, "down_scale", nexp * hidden, dev)

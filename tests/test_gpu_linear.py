@@ -229,3 +229,12 @@ def test_linear_activations_of_huge_values(pkg, dev):
         assert (got[4:] == 0).all(), act
         inf = torch.full((8,), torch.inf, dtype=BF16, device=dev)
         assert (pkg.ops.linear(x.to(dev), w.to(dev), bias=inf, activation=act) == torch.inf).all(), act
+
+
+def test_rows_and_linear_of_no_columns_are_refused(pkg, dev):
+    w, scalar = torch.zeros(0, dtype=BF16, device=dev), torch.zeros((), dtype=BF16, device=dev)
+    for x in (torch.zeros(3, 0, dtype=BF16, device=dev), scalar):
+        for call in (lambda: pkg.ops.quantize_rows(x), lambda: pkg.ops.add_rms_fp8(x, None, w, 1e-6),
+                     lambda: pkg.ops.linear(x, torch.zeros(4, 0, dtype=BF16, device=dev))):
+            with pytest.raises(ValueError):
+                call()

@@ -26,6 +26,7 @@ def test_quantize_rows_refusals(pkg):
     _refused(pkg, f(A, 4, 64, B + 4, C, None), b"aligned")
     _refused(pkg, f(A, 4, 64, A + 256, C, None), b"overlap")
     _refused(pkg, f(A, 4, 64, B, B + 252, None), b"overlap")
+    _refused(pkg, f(A, 2**26, 64, B, C, None), b"rows")
     assert f(None, 0, 64, None, None, None) == 0
 
 
