@@ -289,9 +289,9 @@ template <int MODE, int NA, int NB, int W>
 struct TileShape {
   static constexpr int kWM = W / 2;  // waves side by side along the weight rows
   static constexpr int kWRows = 16 * NA * kWM, kTRows = 32 * NB;
-  // Small tiles, whose fragments of a step fit in registers twice. Stages: as many as leave two workgroups
-  // a CU.
-  static constexpr bool kFlat = W == 4 && NA * NB <= 8;
+  // Small tiles, whose fragments of a step fit in registers twice. Four stages where they fit (256 x 2048 x
+  // 8192 bf16 by 128 x 64: 15.6 us with three, 14.5 with four; by 64 x 64, which share a CU, six take 20).
+  static constexpr bool kFlat = W * NA * NB <= 32;
   static constexpr int kSA = kFlat && NA == 2 ? 4 : 3, kSB = kFlat ? kSA : 2;
   static constexpr bool kScaled = MODE == kRowsDown;
   static constexpr int kAStage = kWRows * 128;
@@ -1031,10 +1031,11 @@ bool tile_fits(RowsMode mode, const RowsGemm& a) {
 // N = 4096, so that there are enough workgroups (one token, N = 2048 bf16: 5.5 us, 7.1 with 32), above
 // it 32, whose token loads are half (16 tokens, N = 8192 e4m3: 8.3, 9.1 with 16).
 //
-// Above that the tile of 64, 128 or 256 squared that takes the least time by its turns: a 256 tile has a
-// CU to itself and takes 54 us of K = 2048 bf16; of the smaller two or more share a CU, 17.5 and 7.7 us
-// each, at least one and 1.4 of them one after the other. (us, 64 / 128 / 256, K = 2048 bf16: 1024 x 2048
-// 17.3, 18.7, -; 2048 x 2048 30.7, 21.2, 48; 1024 x 8192 -, 38.8, 50.4; 2048 x 8192 -, 71.2, 58.7.)
+// Above that the tile that takes the least time by its turns (us of K = 2048 bf16): 256 squared, a CU each,
+// 54 a turn; 128 squared, 17.5, two on a CU; 128 weight rows by 64 token rows, a CU each, 12; 64 squared, 7.3,
+// several on a CU. (64 / 128 by 64 / 128 / 256 squared: 200 x 2048 10.1, 12.5, -, -; 1111 x 1537 16.7, 14.4,
+// 17.5, -; 256 x 8192 17.1, 14.5, -, -; 2048 x 2048 30.7, -, 21.2, 48; 1024 x 8192 -, -, 38.8, 50.4; 2048 x
+// 8192 -, -, 71.2, 58.7.)
 template <int ES>
 hipError_t launch_linear(const RowsGemm& a, hipStream_t s) {
   const bool fits = tile_fits(kRowsLinear, a);
@@ -1043,13 +1044,15 @@ hipError_t launch_linear(const RowsGemm& a, hipStream_t s) {
     return a.N > 4096 ? launch_few<ES, kRowsLinear, 2, 1, 8, 2>(a, s)
                       : launch_few<ES, kRowsLinear, 1, 1, 8, 4>(a, s);
   }
-  auto turns = [&](long long b) {
-    return (double)(((a.M + b - 1) / b) * ((a.N + b - 1) / b)) / 256;
+  auto turns = [&](long long n, long long m) {
+    return (double)(((a.M + m - 1) / m) * ((a.N + n - 1) / n)) / 256;
   };
-  const double c64 = 7.7 * std::max(1.4, turns(64)), c128 = 17.5 * std::max(1.0, turns(128)),
-               c256 = 54 * std::ceil(turns(256));
-  if (c256 <= c128 && c256 <= c64) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
-  if (c128 <= c64) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
+  const double c64 = 7.3 * std::max(1.0, turns(64, 64)), c12864 = 12 * std::ceil(turns(128, 64)),
+               c128 = 17.5 * std::max(1.0, turns(128, 128)), c256 = 54 * std::ceil(turns(256, 256));
+  const double least = std::min(std::min(c64, c12864), std::min(c128, c256));
+  if (c256 == least) return launch_tile<ES, kRowsLinear, 8, 8>(a, s);
+  if (c128 == least) return launch_tile<ES, kRowsLinear, 4, 4>(a, s);
+  if (c12864 == least) return launch_tile<ES, kRowsLinear, 2, 2, 8>(a, s);
   return launch_tile<ES, kRowsLinear, 2, 2>(a, s);
 }
 

@@ -22,10 +22,10 @@ def _small(dev, g, *shape, e4m3=False):
 
 
 
-# 256 x 256 tiles: one round of workgroups, two; 128: few, more than two a unit; 64: few, more than four
-# a unit, either way round
+# 256 x 256 tiles: one round of workgroups, two; 128: few, more than two a unit; 64: few, more than two a
+# unit, either way round; 128 x 64
 TILES = [(4096, 4096, 48), (7700, 4000, 32), (7700, 4001, 448), (1100, 2100, 200), (4200, 4000, 48), (300, 520, 328),
-         (40, 66001, 80), (66001, 40, 144), (33, 77, 16)]
+         (40, 66001, 80), (66001, 40, 144), (33, 77, 16), (1111, 1537, 328), (250, 8000, 104)]
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
