@@ -187,7 +187,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // operands staged in LDS. Wave (wm, wn) owns 16 NA weight rows and every other 16-row token block:
 // 16 x 16 blocks acc[NA][NB], so each fragment read from LDS feeds NA or NB matrix instructions (at NA =
 // NB = 8 the reads of a step take half the time of its products; with 64 x 128 blocks, three quarters).
-// Linear: four waves, a SIMD's whole register file each, since the products are the bound (8192^2, K =
+// Linear's larger tiles: four waves, a SIMD's whole register file each, since the products are the bound (8192^2, K =
 // 2048 bf16 270 us, 273 with eight waves; K = 4096 e4m3 220 and 229). The experts' larger tiles wait for
 // memory and take long in their epilogue: eight waves, which wait in turns (4096 tokens as below 299 ->
 // 276 us).
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // ends with 4 NA neighbouring outputs (or 2 NA gate and 2 NA up ones) of each token
 // and stores them in 16-byte pieces.
 //
-// A step's products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0). Between
+// A larger tile's step: its products go in four quarters (weight half, token half): (0, 0), (0, 1), (1, 1), (1, 0). Between
 // its matrix instructions, which leave three of four issue slots free, each reads from LDS, early, the
 // half that the next one needs; the last two read the next step's first halves, the tokens' into the
 // registers that held half 1. Two barriers a step. After the first quarter the step's tokens have been
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
 // and the reads after each block's products, a step of 256 x 256 took 4400 cycles; its products
 // take 2048.)
 //
-// A workgroup walks over tiles, as many workgroups as the chip holds. The next tile's first two steps
+// A workgroup walks over tiles, as many workgroups as the chip holds. The next tile's first steps
 // are requested before the present one's epilogue, which needs only the last weight stage of LDS, so
 // that memory is not idle meanwhile.
 struct Frag {
