@@ -503,7 +503,13 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
         sc[i] >>= 8 * kq;
       }
     }
-    if (SC) asm volatile("s_nop 3");  // before a product reads them
+    // Two wait states between the last shift and a product that reads it: the compiler keeps them for
+    // products of its own, not for asm. The ties hold the shifts in front of the wait.
+    if (SC) {
+#pragma unroll
+      for (int i = 0; i < FB; ++i) asm volatile("" : "+v"(sc[i]));
+      asm volatile("s_nop 1");
+    }
   };
   // One quarter: weight half x, token half y. After its product p (bf16: all first halves, then all
   // second ones, so that no product waits for the one before), what falls due: read k of NR at
