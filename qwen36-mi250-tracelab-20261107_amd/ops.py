@@ -542,8 +542,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
     if not _rows_in_place(w, k, size):
         raise ValueError("rows of w must be contiguous and start at multiples of 16 bytes")
     if kind is FP8:
-        x_scale = _vector(x_scale, _F32, "x_scale", rows, dev).data_ptr()
-        w_scale = _vector(w_scale, _F32, "w_scale", n, dev).data_ptr()
+        x_scale = _vector(x_scale, _F32, "x_scale", rows, dev)  # may be copies: kept until the call
+        w_scale = _vector(w_scale, _F32, "w_scale", n, dev)
     elif x_scale is not None or w_scale is not None:
         raise ValueError("bf16 operands take no scales")
     _sizes("linear", rows, n, k)
@@ -561,8 +561,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
             raise ValueError(f"residual has shape {tuple(residual.shape)}, the output {out_shape}")
         residual = _input(residual, torch.bfloat16, "residual", dev)
     out = torch.empty(out_shape, dtype=torch.bfloat16, device=x.device)
-    _call("linear", dev, _lib.load().moe_linear, x.data_ptr(), ldx, x_scale, w.data_ptr(),
-          w.stride(0) if n > 1 else k, w_scale,
+    _call("linear", dev, _lib.load().moe_linear, x.data_ptr(), ldx, ptr(x_scale), w.data_ptr(),
+          w.stride(0) if n > 1 else k, ptr(w_scale),
           _lib.WEIGHTS_FP8_E4M3 if size == 1 else _lib.WEIGHTS_BF16, rows, k, n, ptr(bias), bias_f32,
           act, ptr(mul), ptr(residual), out.data_ptr())
     return out
