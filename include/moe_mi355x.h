@@ -268,9 +268,10 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
                void* stream);
 
 /* Routed experts on 8-bit rows q [T, H] with x_scale [T]: per pair (t, j) of top_k_index [T, k]
- * (each in [0, E)) a = silu(gate) * up in fp32, in e4m3 with one power-of-two scale per 32
- * columns (the least with amax <= 448 scale); y = a . down, kept in fp32 for few pairs (16, or E / 4),
- * else in fp16 with a power of two per 32 columns; out [T, H] = bf16(sum_j top_k_weights[t, j] y_tj).
+ * (in [0, E); others count as the nearest) a = silu(gate) * up in fp32, in e4m3 with one
+ * power-of-two scale per 32 columns (the least with amax <= 448 scale); y = a . down, kept in fp32
+ * for few pairs (16, or E / 4), else in fp16 with a power of two per 32 columns;
+ * out [T, H] = bf16(sum_j top_k_weights[t, j] y_tj).
  * With shared [T, H] and its gate's logits (one bf16 per token, ld_gate elements apart) and with
  * residual [T, H] (each may be null), out goes on as moe_combine does:
  * bf16(bf16(out + bf16(bf16(sigmoid(gate)) * shared)) + residual).

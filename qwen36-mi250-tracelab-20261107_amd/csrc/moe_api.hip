@@ -1263,7 +1263,7 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
             "sort launch");
     a.table = w.table, a.order = w.order, a.MT = w.MT;
   } else {
-    a.ids = top_k_index;
+    a.ids = top_k_index, a.E = E;
   }
   HIP_TRY(launch_rows_gemm(kRowsGateUp, 1, a, w.bm, s), "gate_up launch");
   a.x = w.aq, a.ldx = I;

@@ -61,6 +61,7 @@ struct RowsGemm {
   uint8_t* yexp;      // [P, N / 32]: exponent + 128 of 32 values of y
   // a few pairs (kRowsGateUp without a table, launch_rows_pairs_down): pair p is its own sorted row
   const long long* ids;
+  int E;              // experts
   const uint16_t* wts;
 };
 
@@ -77,6 +78,12 @@ __device__ __forceinline__ float rows_tail(const RowsTail& t, float sum, float g
                                            float res) {
   if (t.shared) sum = rbf(rbf(sum) + rbf(gate * shared));
   return t.res ? rbf(sum) + res : sum;
+}
+
+// Pair p's expert, ids outside [0, E) as the nearest in it: what the sort makes of them.
+__device__ __forceinline__ int rows_pair_expert(const RowsGemm& a, long long p) {
+  const long long v = a.ids[p];
+  return (int)(v < 0 ? 0 : (v >= a.E ? a.E - 1 : v));
 }
 
 typedef int v8i_t __attribute__((ext_vector_type(8)));

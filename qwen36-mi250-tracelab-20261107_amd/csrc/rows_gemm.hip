@@ -25,7 +25,7 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
     return t.r0 < a.M;
   }
   if (MODE == kRowsGateUp && a.ids) {
-    t.e = (int)a.ids[tile];
+    t.e = rows_pair_expert(a, tile);
     t.r0 = tile;
     t.r1 = tile + 1;
     return true;
@@ -858,7 +858,7 @@ __global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a,
   float total[4] = {0.f, 0.f, 0.f, 0.f};
   for (int j = wave; j < a.topk; j += kPairWaves) {
     const long long p = (long long)blockIdx.y * a.topk + j;
-    const long long e = a.ids[p];
+    const long long e = rows_pair_expert(a, p);
     const uint8_t* wp = a.w + e * a.estride + (n0 + lr) * a.ldw;
     const uint8_t* xp = a.x + p * a.ldx;  // every column of the product is the pair's row
     const float w = bf_bits2f(a.wts[p]);

@@ -587,7 +587,8 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
     products on the e4m3 matrix instructions. Between them a = silu(gate) * up, fp32, goes in e4m3
     with one power-of-two scale per 32 columns. The pairs' outputs meet in fp32 (few pairs) or through
     fp16 with a power of two per 32 columns; their weighted sum, fp32 with bf16 weights, is
-    rounded to bf16. ``top_k_index`` [T, k] int64 holds experts in [0, E). ``shared`` [T, H] with
+    rounded to bf16. ``top_k_index`` [T, k] int64 holds experts in [0, E); as in the other operators others
+    count as the nearest (a masked slot's -1 or E, with weight 0, is harmless). ``shared`` [T, H] with
     ``shared_gate_logit`` [T] and ``residual`` [T, H], bf16, are added as ``combine`` adds them."""
     if not (q.is_cuda and gate_up.is_cuda and down.is_cuda and top_k_index.is_cuda):
         _need_cuda(q, gate_up, down, top_k_index)
