@@ -1186,7 +1186,7 @@ int moe_linear(const void* x, long long ldx, const float* x_scale, const void* w
   CHECK_ARG(x && w && out, "linear: null pointer");
   CHECK_ARG((es == 1) == (x_scale != nullptr) && (es == 1) == (w_scale != nullptr),
             "linear: e4m3 operands take x_scale and w_scale, bf16 ones neither");
-  CHECK_ARG(ldx >= K && ldw >= K && ldx * es <= (1 << 22) && ldw * es <= (1 << 22),
+  CHECK_ARG(ldx >= K && ldw >= K && ldx <= (1 << 22) / es && ldw <= (1 << 22) / es,
             "linear: ldx and ldw must be >= K and at most 4 MiB");
   const long long n = 2LL * M * N;
   const Span in[] = {{x, ((M - 1) * ldx + K) * es}, {w, ((N - 1) * ldw + K) * es},
