@@ -1230,7 +1230,8 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
   CHECK_ARG(q && x_scale && top_k_index && top_k_weights && gate_up && gu_scale && down &&
                 dn_scale && out,
             "experts_fp8: null pointer");
-  CHECK_ARG(!shared || (shared_gate && ld_gate >= 0), "experts_fp8: shared needs its gate's logits");
+  CHECK_ARG(!shared || (shared_gate && ld_gate >= 0 && ld_gate < (1LL << 31)),
+            "experts_fp8: shared needs its gate's logits, less than 2^31 elements apart");
   CHECK_ARG(((uintptr_t)q | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)shared |
              (uintptr_t)residual | (uintptr_t)out | (uintptr_t)workspace) % 16 == 0,
             "experts_fp8: q, the weights, shared, residual, out and the workspace must be 16-byte aligned");
@@ -1240,9 +1241,10 @@ int moe_experts_fp8_forward(const void* q, const float* x_scale, int T, int H, i
   const long long row = 2LL * T * H, pairs = (long long)T * k, proj = (long long)E * H * I;
   const Span in[] = {{q, row / 2}, {x_scale, 4LL * T}, {top_k_index, 8 * pairs},
                      {top_k_weights, 2 * pairs}, {gate_up, 2 * proj}, {gu_scale, 8LL * E * I},
-                     {down, proj}, {dn_scale, 4LL * E * H}, {shared, row}, {residual, row}};
+                     {down, proj}, {dn_scale, 4LL * E * H}, {shared, row}, {residual, row},
+                     {shared ? shared_gate : nullptr, shared ? 2 * ((T - 1) * ld_gate + 1) : 0}};
   const Span o[] = {{out, row}, {workspace, (long long)w.bytes}};
-  CHECK_ARG(apart(in, 10, o, 2),
+  CHECK_ARG(apart(in, 11, o, 2),
             "experts_fp8: out and the workspace must not overlap the inputs or each other");
   hipStream_t s = (hipStream_t)stream;
   const uint16_t* wts = static_cast<const uint16_t*>(top_k_weights);
