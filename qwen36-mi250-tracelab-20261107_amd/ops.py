@@ -28,6 +28,7 @@ caching allocator; weights are read in place. Nothing here synchronises with the
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -438,11 +439,19 @@ def _input(t: torch.Tensor, dtype: torch.dtype, name: str, dev: int | None = Non
     return t.clone() if t.data_ptr() & 15 else t
 
 
-def _vector(t: torch.Tensor | None, dtypes: tuple, name: str, n: int, dev: int) -> torch.Tensor:
-    if t is None or t.dtype not in dtypes or t.numel() != n or t.get_device() != dev:
+def _vector(t: torch.Tensor | None, dtypes: tuple, name: str, shape: tuple, dev: int) -> torch.Tensor:
+    """``t`` contiguous, of ``shape`` up to dimensions of one, or flat."""
+    if (t is None or t.dtype not in dtypes or t.get_device() != dev
+            or (t.shape != shape and not _same_order(t.shape, shape))):
         kind = " or ".join(str(d) for d in dtypes)
-        raise ValueError(f"{name} must be {n} {kind} values on cuda:{dev}")
+        got = None if t is None else f"{t.dtype} {tuple(t.shape)} on {t.device}"
+        raise ValueError(f"{name} must be {kind} {tuple(shape)} on cuda:{dev} (got {got})")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _same_order(got: tuple, shape: tuple) -> bool:
+    got, shape = [d for d in got if d != 1], [d for d in shape if d != 1]
+    return got == shape or (len(got) < 2 and math.prod(got) == math.prod(shape))
 
 
 def _call(name: str, dev: int, fn, *args) -> None:
@@ -542,15 +551,15 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
     if not _rows_in_place(w, k, size):
         raise ValueError("rows of w must be contiguous and start at multiples of 16 bytes")
     if kind is FP8:
-        x_scale = _vector(x_scale, _F32, "x_scale", rows, dev)  # may be copies: kept until the call
-        w_scale = _vector(w_scale, _F32, "w_scale", n, dev)
+        x_scale = _vector(x_scale, _F32, "x_scale", shape[:-1], dev)  # may be copies: kept until the call
+        w_scale = _vector(w_scale, _F32, "w_scale", (n,), dev)
     elif x_scale is not None or w_scale is not None:
         raise ValueError("bf16 operands take no scales")
     _sizes("linear", rows, n, k)
     out_shape = (*shape[:-1], n)
     bias_f32 = 0
     if bias is not None:
-        bias = _vector(bias, _BIAS, "bias", n, dev)
+        bias = _vector(bias, _BIAS, "bias", (n,), dev)
         bias_f32 = int(bias.dtype is torch.float32)
     if mul is not None:
         if mul.shape != out_shape:
@@ -616,9 +625,9 @@ def experts_fp8(q: torch.Tensor, scale: torch.Tensor, top_k_index: torch.Tensor,
             raise ValueError(f"{name} is on {t.device}, q on {q.device}")
     top_k = top_k_index.shape[1]
     _sizes("experts_fp8", tokens, hidden, nexp, two_i)
-    scale = _vector(scale, _F32, "scale", tokens, dev)
-    gus = _vector(gate_up_scale, _F32, "gate_up_scale", nexp * two_i, dev)
-    dns = _vector(down_scale, _F32, "down_scale", nexp * hidden, dev)
+    scale = _vector(scale, _F32, "scale", (tokens,), dev)
+    gus = _vector(gate_up_scale, _F32, "gate_up_scale", (nexp, two_i), dev)
+    dns = _vector(down_scale, _F32, "down_scale", (nexp, hidden), dev)
     idx = top_k_index if top_k_index.is_contiguous() else top_k_index.contiguous()
     wts = top_k_weights.to(torch.bfloat16).contiguous()
     ld_gate = 0

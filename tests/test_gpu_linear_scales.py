@@ -63,3 +63,41 @@ def test_linear_strided_scales_in_a_graph(pkg, dev):
         torch.cuda.synchronize()
         assert torch.equal(out, pkg.ops.linear(x, w, x_scale=xv.contiguous(), w_scale=ws, mul=mul)), i
         torch.cuda.synchronize()
+
+
+def test_scales_of_another_shape_are_refused(pkg, dev):
+    """As many values in another order would be taken for the wrong rows; one dimension, and dimensions
+    of one, leave the order as it is."""
+    x, w, xs, ws, bias, _, _ = _operands(6, 64, 8, dev)
+    lin, x3 = pkg.ops.linear, x.view(2, 3, 64)
+    want = lin(x, w, x_scale=xs, w_scale=ws)
+    for a, b in ((xs.view(2, 3), ws), (xs, ws), (xs.view(2, 3, 1), ws.view(8, 1)), (xs.view(1, 6), ws.view(1, 8))):
+        assert torch.equal(lin(x3, w, x_scale=a, w_scale=b).view(6, 8), want)
+    one = lin(x[0], w, x_scale=xs[0], w_scale=ws)
+    assert torch.equal(one, want[0]) and torch.equal(lin(x[:1], w, x_scale=xs[:1, None], w_scale=ws)[0], one)
+    for bad in (dict(x_scale=xs.view(3, 2), w_scale=ws), dict(x_scale=xs.view(2, 3), w_scale=ws.view(2, 4)),
+                dict(x_scale=xs.view(2, 3).t(), w_scale=ws), dict(x_scale=xs, w_scale=ws, bias=bias.view(4, 2))):
+        with pytest.raises(ValueError):
+            lin(x3, w, **bad)
+
+
+def test_expert_scales_of_another_shape_are_refused(pkg, dev):
+    T, H, E, I = 5, 64, 8, 32
+    g = torch.Generator().manual_seed(0)
+    q, xs = ref.rows(torch.randn(T, H, generator=g).to(BF16))
+    gu, gus = ref.rows(torch.randn(E, 2 * I, H, generator=g).to(BF16))
+    dn, dns = ref.rows(torch.randn(E, H, I, generator=g).to(BF16))
+    idx, wts = torch.randint(E, (T, 2), generator=g), torch.rand(T, 2, generator=g).to(BF16)
+    q, xs, gu, gus, dn, dns, idx, wts = (t.to(dev) for t in (q, xs, gu, gus, dn, dns, idx, wts))
+
+    def call(scale=xs, gate_up_scale=gus, down_scale=dns):
+        return pkg.ops.experts_fp8(q, scale, idx, wts, gu, dn, gate_up_scale=gate_up_scale, down_scale=down_scale)
+
+    want = call()
+    for good in (dict(scale=xs[:, None]), dict(gate_up_scale=gus.flatten()), dict(down_scale=dns[..., None]),
+                 dict(gate_up_scale=_spread(gus), down_scale=_spread(dns), scale=_spread(xs))):
+        assert torch.equal(call(**good), want)
+    for bad in (dict(gate_up_scale=gus.t()), dict(gate_up_scale=gus.t().contiguous()), dict(down_scale=dns.t()),
+                dict(gate_up_scale=gus.view(2 * E, I)), dict(down_scale=dns.view(E, 2, H // 2))):
+        with pytest.raises(ValueError):
+            call(**bad)
