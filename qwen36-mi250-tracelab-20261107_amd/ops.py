@@ -117,9 +117,8 @@ def router_logits(x: torch.Tensor, w_pack: torch.Tensor) -> torch.Tensor:
     tokens, hidden = x.shape
     n_pack = w_pack.shape[0]
     out = torch.empty((tokens, n_pack), dtype=torch.bfloat16, device=x.device)
-    lib = _lib.load()
-    check(lib.moe_router_logits(ptr(x), tokens, hidden, ptr(w_pack), n_pack, ptr(out), stream_of(x)),
-          "router_logits")
+    _call("router_logits", x.get_device(), _lib.load().moe_router_logits, ptr(x), tokens, hidden,
+          ptr(w_pack), n_pack, ptr(out))
     return out
 
 
