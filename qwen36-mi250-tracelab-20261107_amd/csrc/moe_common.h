@@ -106,22 +106,22 @@ __device__ __forceinline__ bf16x8_t as_bf16x8(uint4 v) {
 }
 
 // 16 OCP e4m3fn bytes -> two bf16x8 operands (exact: every e4m3 value is a bf16 value).
-// gfx950's scaled conversion with scale 1.0 turns two e4m3 bytes into two bf16 in one step.
+// gfx950's scaled conversion turns two e4m3 bytes, times a power of two, into two bf16 in one step.
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 template <bool HI>
-__device__ __forceinline__ uint32_t fp8x2_to_bf16x2(uint32_t w) {
-  bf16x2_t r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI);
+__device__ __forceinline__ uint32_t fp8x2_to_bf16x2(uint32_t w, float two = 1.0f) {
+  bf16x2_t r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, two, HI);
   return __builtin_bit_cast(uint32_t, r);
 }
-__device__ __forceinline__ void fp8x16_to_bf16(uint4 q, uint4& lo, uint4& hi) {
-  lo.x = fp8x2_to_bf16x2<false>(q.x);
-  lo.y = fp8x2_to_bf16x2<true>(q.x);
-  lo.z = fp8x2_to_bf16x2<false>(q.y);
-  lo.w = fp8x2_to_bf16x2<true>(q.y);
-  hi.x = fp8x2_to_bf16x2<false>(q.z);
-  hi.y = fp8x2_to_bf16x2<true>(q.z);
-  hi.z = fp8x2_to_bf16x2<false>(q.w);
-  hi.w = fp8x2_to_bf16x2<true>(q.w);
+__device__ __forceinline__ void fp8x16_to_bf16(uint4 q, uint4& lo, uint4& hi, float two = 1.0f) {
+  lo.x = fp8x2_to_bf16x2<false>(q.x, two);
+  lo.y = fp8x2_to_bf16x2<true>(q.x, two);
+  lo.z = fp8x2_to_bf16x2<false>(q.y, two);
+  lo.w = fp8x2_to_bf16x2<true>(q.y, two);
+  hi.x = fp8x2_to_bf16x2<false>(q.z, two);
+  hi.y = fp8x2_to_bf16x2<true>(q.z, two);
+  hi.z = fp8x2_to_bf16x2<false>(q.w, two);
+  hi.w = fp8x2_to_bf16x2<true>(q.w, two);
 }
 
 __device__ __forceinline__ f32x4_t mfma16x16x32(uint4 a, uint4 b, f32x4_t c) {

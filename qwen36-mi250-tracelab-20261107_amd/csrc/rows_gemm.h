@@ -17,7 +17,10 @@
 // Sums are fp32, but the e4m3 instruction brings the products of eight neighbouring k to the exponent
 // of their largest and cuts, towards zero, what lies below 2^-13 of it (measured: beside 2^16, 12
 // counts as 8 and 7 as 0). Only products under 2^-6 of the largest lose anything. That is the
-// price of its rate, twice the bf16 instruction's.
+// price of its rate, twice the bf16 instruction's: kRowsLinear's sums are off by some 2e-4 of their size, a
+// tenth of the result's rounding; the experts' values between the products are rounded to e4m3 next, where
+// as little puts some on the neighbouring value (4096 tokens: outputs off by 2.0e-3 of their size, 1.7e-3
+// with every product kept). With few rows every product is kept (rows_mma_wide).
 // Weights are the A operand and tokens the B operand: lane (lr, kq) ends with four neighbouring
 // outputs n = 4 kq .. 4 kq + 3 of token lr per 16 x 16 block.
 #pragma once
@@ -98,14 +101,28 @@ __device__ __forceinline__ f32x4_t rows_mma(uint4 a0, uint4 a1, uint4 b0, uint4 
                    (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
-// The same for e4m3 with token lr's values 32 kq .. 32 kq + 31 of the step times 2^(sb - 127).
-__device__ __forceinline__ f32x4_t rows_mma_scaled(uint4 a0, uint4 a1, uint4 b0, uint4 b1, int sb,
-                                                   f32x4_t c) {
-  const v8i_t a = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w,
-                   (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
-  const v8i_t b = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w,
-                   (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f, 0, sb);
+// The same for e4m3 with every product kept: widened to bf16, which holds e4m3 values exactly, token lr's
+// times two0 and two1, the powers of two of their groups of 32 columns. Half the rate, and as many conversions
+// as values: for few rows, where memory is the bound (H = 2048, I = 512, 256 experts, us a call with the e4m3
+// instruction / so: 8 tokens 40.4, 40.4; 64 141.8, 141.5; 384 201.5, 199.9; linear 16 x 8192 x 8192 16.4,
+// 16.5). At 32 tokens the experts' output was off by 1.9e-3 of its size, and is by 1.7e-3, the last rounding
+// alone.
+__device__ __forceinline__ f32x4_t rows_mma_wide(uint4 a0, uint4 a1, uint4 b0, uint4 b1, float two0,
+                                                 float two1, f32x4_t c) {
+  uint4 al, ah, bl, bh;
+  fp8x16_to_bf16(a0, al, ah);
+  fp8x16_to_bf16(b0, bl, bh, two0);
+  c = mfma16x16x32(ah, bh, mfma16x16x32(al, bl, c));
+  fp8x16_to_bf16(a1, al, ah);
+  fp8x16_to_bf16(b1, bl, bh, two1);
+  return mfma16x16x32(ah, bh, mfma16x16x32(al, bl, c));
+}
+// The scales of the four groups of 32 columns of a step of 128 of sorted row r; group g's, 2^(byte - 127).
+__device__ __forceinline__ uint32_t rows_group_scales(const RowsGemm& a, int step, long long r) {
+  return reinterpret_cast<const uint32_t*>(a.asc)[step * a.P + r];
+}
+__device__ __forceinline__ float rows_group_two(uint32_t scales, int g) {
+  return __uint_as_float((scales >> (8 * g) & 0xffu) << 23);
 }
 
 // v sigmoid(t), as v / (1 + e) or v e / (1 + e) with e = exp(-|t|) <= 1, from the hardware's exp2 and

@@ -44,6 +44,8 @@ __device__ __forceinline__ bool rows_tile(const RowsGemm& a, int tile, int tile_
 // by its latency (2048 x 2048 bf16 5.4 us).
 template <int ES, int MODE, int NB, int MB, int W, int U>
 __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
+  // linear of 17 to 32 e4m3 rows has products enough to notice (17 x 4096 x 16384: 16.9 us, wide 18.7)
+  constexpr bool WIDE = ES == 1 && !(MODE == kRowsLinear && MB > 1);
   __shared__ f32x4_t red[W][NB * MB][64];
   RowsTile t;
   if (!rows_tile<MODE>(a, a.tile0 + blockIdx.y, 16 * MB, t)) return;
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
   const int c0 = (int)((long long)nch * wave / W), c1 = (int)((long long)nch * (wave + 1) / W);
   for (int c = c0; c < c1; c += U) {
     uint4 wv[U][NB][2], xv[U][MB][2];
-    int sv[U][MB];
+    uint32_t sv[U][MB];
 #pragma unroll
     for (int s = 0; s < U; ++s) {
       // past the wave's part or the row's end: bytes there again, below made zeros
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
       for (int m = 0; m < MB; ++m) {
         xv[s][m][0] = ld16(xp[m] + o0);
         xv[s][m][1] = ld16(xp[m] + o1);
-        if (MODE == kRowsDown) sv[s][m] = a.asc[(min(c + s, nch - 1) * a.P + row[m]) * 4 + kq];
+        if (MODE == kRowsDown) sv[s][m] = rows_group_scales(a, min(c + s, nch - 1), row[m]);
       }
     }
 #pragma unroll
@@ -143,10 +145,14 @@ __global__ __launch_bounds__(W * 64) void k_rows_few(RowsGemm a) {
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int m = 0; m < MB; ++m)
-          acc[b][m] = MODE == kRowsDown
-                          ? rows_mma_scaled(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1],
-                                            sv[s][m], acc[b][m])
-                          : rows_mma<ES>(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1], acc[b][m]);
+          if constexpr (MODE == kRowsDown)
+            acc[b][m] = rows_mma_wide(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1],
+                                      rows_group_two(sv[s][m], kq >> 1),
+                                      rows_group_two(sv[s][m], 2 + (kq >> 1)), acc[b][m]);
+          else if constexpr (WIDE)
+            acc[b][m] = rows_mma_wide(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1], 1.f, 1.f, acc[b][m]);
+          else
+            acc[b][m] = rows_mma<ES>(wv[s][b][0], wv[s][b][1], xv[s][m][0], xv[s][m][1], acc[b][m]);
     }
   }
 #pragma unroll
@@ -870,21 +876,22 @@ __global__ __launch_bounds__(kPairWaves * 64) void k_rows_pairs_down(RowsGemm a,
     constexpr int U = 4;
     for (int c = 0; c < nch; c += U) {
       uint4 wv[U][2], xv[U][2];
-      int sv[U];
+      uint32_t sv[U];
 #pragma unroll
       for (int s = 0; s < U; ++s) {
         const int k0 = (c + s) * 128 + kq * 16;
         const int o0 = min(k0, a.Kb - 16), o1 = min(k0 + 64, a.Kb - 16);
         wv[s][0] = ld16_stream(wp + o0), wv[s][1] = ld16_stream(wp + o1);
         xv[s][0] = ld16(xp + o0), xv[s][1] = ld16(xp + o1);
-        sv[s] = a.asc[(min(c + s, nch - 1) * a.P + p) * 4 + kq];
+        sv[s] = rows_group_scales(a, min(c + s, nch - 1), p);
       }
 #pragma unroll
       for (int s = 0; s < U; ++s) {
         const int k0 = (c + s) * 128 + kq * 16;
         if (k0 >= a.Kb) xv[s][0] = make_uint4(0u, 0u, 0u, 0u);
         if (k0 + 64 >= a.Kb) xv[s][1] = make_uint4(0u, 0u, 0u, 0u);
-        acc = rows_mma_scaled(wv[s][0], wv[s][1], xv[s][0], xv[s][1], sv[s], acc);
+        acc = rows_mma_wide(wv[s][0], wv[s][1], xv[s][0], xv[s][1], rows_group_two(sv[s], kq >> 1),
+                            rows_group_two(sv[s], 2 + (kq >> 1)), acc);
       }
     }
 #pragma unroll
