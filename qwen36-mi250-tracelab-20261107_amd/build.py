@@ -48,6 +48,8 @@ def _compile(src: Path) -> Path:
     err = "\n".join(line for line in res.stderr.splitlines() if noise not in line)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src.name}:\n{err}")
+    if "warning:" in err:
+        print(err, file=sys.stderr)
     return obj
 
 

@@ -230,8 +230,8 @@ AuxStream* aux_stream(hipStream_t caller) {
   }
   if (hipEventCreateWithFlags(&a.fork, hipEventDisableTiming) != hipSuccess ||
       hipEventCreateWithFlags(&a.join, hipEventDisableTiming) != hipSuccess) {
-    if (a.fork) hipEventDestroy(a.fork);
-    hipStreamDestroy(a.s);
+    if (a.fork) (void)hipEventDestroy(a.fork);
+    (void)hipStreamDestroy(a.s);
     a.s = nullptr;
     return nullptr;
   }

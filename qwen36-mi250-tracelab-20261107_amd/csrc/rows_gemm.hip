@@ -559,36 +559,38 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   // Step d with its tokens' half 0 in p; half 1 goes to q, and the next step's half 0 after it.
   auto step = [&](int d, Frag (&p)[FB], uint32_t (&sp)[FB], Frag (&q)[FB], uint32_t (&sq)[FB])
                   __attribute__((always_inline)) {
-    const uint32_t at = aaddr + ra[0], at1 = aaddr + ra[1];
-    quarter(a0, p, sp, c0, c0, chb, [&](auto k) __attribute__((always_inline)) {
-      constexpr int K = decltype(k)::value;
-      read_b(rb[0], integral_constant<int, HB + K>{}, q[K], sq[K]);
-    }, c0, none);
-    lds_frags_ready();
-    ready_b(q, sq);
-    wait_loads(LA + NLB);  // in flight: step d + 1's tokens, step d + 2's weights
-    __builtin_amdgcn_s_barrier();
-    const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
-    quarter(a0, q, sq, c0, c1, cha, [&](auto k) __attribute__((always_inline)) {
-      constexpr int K = decltype(k)::value;
-      read_a(at, integral_constant<int, HA + K>{}, a1[K]);
-    }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb, k); });
-    lds_frags_ready();
-    ready_a(a1);
-    quarter(a1, q, sq, c1, c1, cha, [&](auto k) __attribute__((always_inline)) {
-      read_a(at1, k, a0[decltype(k)::value]);
-    }, c0, none);
-    lds_frags_ready();
-    ready_a(a0);
-    wait_loads(LA + NLB);  // in flight: step d + 2's weights and tokens
-    __builtin_amdgcn_s_barrier();
-    quarter(a1, p, sp, c1, c0, chb, [&](auto k) __attribute__((always_inline)) {
-      constexpr int K = decltype(k)::value;
-      read_b(rb[1], k, q[K], sq[K]);
-    }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na, k); });
-    lds_frags_ready();
-    ready_b(q, sq);
-    turn(ra), turn(rb);
+    if constexpr (!FLAT) {
+      const uint32_t at = aaddr + ra[0], at1 = aaddr + ra[1];
+      quarter(a0, p, sp, c0, c0, chb, [&](auto k) __attribute__((always_inline)) {
+        constexpr int K = decltype(k)::value;
+        read_b(rb[0], integral_constant<int, HB + K>{}, q[K], sq[K]);
+      }, c0, none);
+      lds_frags_ready();
+      ready_b(q, sq);
+      wait_loads(LA + NLB);  // in flight: step d + 1's tokens, step d + 2's weights
+      __builtin_amdgcn_s_barrier();
+      const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
+      quarter(a0, q, sq, c0, c1, cha, [&](auto k) __attribute__((always_inline)) {
+        constexpr int K = decltype(k)::value;
+        read_a(at, integral_constant<int, HA + K>{}, a1[K]);
+      }, integral_constant<int, NLB>{}, [&](auto k) __attribute__((always_inline)) { load_b(nb, k); });
+      lds_frags_ready();
+      ready_a(a1);
+      quarter(a1, q, sq, c1, c1, cha, [&](auto k) __attribute__((always_inline)) {
+        read_a(at1, k, a0[decltype(k)::value]);
+      }, c0, none);
+      lds_frags_ready();
+      ready_a(a0);
+      wait_loads(LA + NLB);  // in flight: step d + 2's weights and tokens
+      __builtin_amdgcn_s_barrier();
+      quarter(a1, p, sp, c1, c0, chb, [&](auto k) __attribute__((always_inline)) {
+        constexpr int K = decltype(k)::value;
+        read_b(rb[1], k, q[K], sq[K]);
+      }, integral_constant<int, LA>{}, [&](auto k) __attribute__((always_inline)) { load_a(na, k); });
+      lds_frags_ready();
+      ready_b(q, sq);
+      turn(ra), turn(rb);
+    }
   };
 
   // A small tile's step: its fragments are in registers (w, tk), the next step's are read to others
@@ -598,39 +600,41 @@ __global__ __launch_bounds__(64 * W, 1) void k_rows_tile(RowsGemm a, int ncol, i
   auto flat_step = [&](int d, const Frag (&w)[FA], const Frag (&tk)[FB], const uint32_t (&sc)[FB],
                        Frag (&wn)[FA], Frag (&tn)[FB], uint32_t (&sn)[FB])
                        __attribute__((always_inline)) {
-    wait_loads((S::kSA - 2) * (LA + NLB));  // step d + 1 has arrived
-    __builtin_amdgcn_s_barrier();
-    const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
-    const uint32_t at = aaddr + ra[1];
-    constexpr int ALL = NA * NB * ES, NL = LA + NLB;
-    static_for<ALL>([&](auto prod) __attribute__((always_inline)) {
-      constexpr int p = decltype(prod)::value, H = p / (NA * NB), i = p / NA % NB, j = p % NA;
-      tile_mma<ES, SC, H>(w[j], tk[i], sc[i], acc[j][i]);
-      __builtin_amdgcn_sched_barrier(0);
-      static_for<NA + NB>([&](auto kc) __attribute__((always_inline)) {
-        constexpr int k = decltype(kc)::value;
-        if constexpr ((k < ALL ? k : ALL - 1) == p) {
-          if constexpr (k < NB)
-            read_b(rb[1], kc, tn[k], sn[k]);
-          else
-            read_a(at, integral_constant<int, k - NB>{}, wn[k - NB]);
-        }
+    if constexpr (FLAT) {
+      wait_loads((S::kSA - 2) * (LA + NLB));  // step d + 1 has arrived
+      __builtin_amdgcn_s_barrier();
+      const Step nb = step_b(d + S::kSB, rb[0]), na = step_a(d + S::kSA, ra[0]);
+      const uint32_t at = aaddr + ra[1];
+      constexpr int ALL = NA * NB * ES, NL = LA + NLB;
+      static_for<ALL>([&](auto prod) __attribute__((always_inline)) {
+        constexpr int p = decltype(prod)::value, H = p / (NA * NB), i = p / NA % NB, j = p % NA;
+        tile_mma<ES, SC, H>(w[j], tk[i], sc[i], acc[j][i]);
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<NA + NB>([&](auto kc) __attribute__((always_inline)) {
+          constexpr int k = decltype(kc)::value;
+          if constexpr ((k < ALL ? k : ALL - 1) == p) {
+            if constexpr (k < NB)
+              read_b(rb[1], kc, tn[k], sn[k]);
+            else
+              read_a(at, integral_constant<int, k - NB>{}, wn[k - NB]);
+          }
+        });
+        static_for<NL>([&](auto kc) __attribute__((always_inline)) {
+          constexpr int k = decltype(kc)::value;
+          if constexpr (k * ALL / NL == p) {
+            if constexpr (k < LA)
+              load_a(na, kc);
+            else
+              load_b(nb, integral_constant<int, k - LA>{});
+          }
+        });
+        __builtin_amdgcn_sched_barrier(0);
       });
-      static_for<NL>([&](auto kc) __attribute__((always_inline)) {
-        constexpr int k = decltype(kc)::value;
-        if constexpr (k * ALL / NL == p) {
-          if constexpr (k < LA)
-            load_a(na, kc);
-          else
-            load_b(nb, integral_constant<int, k - LA>{});
-        }
-      });
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    lds_frags_ready();
-    ready_a(wn);
-    ready_b(tn, sn);
-    turn(ra), turn(rb);
+      lds_frags_ready();
+      ready_a(wn);
+      ready_b(tn, sn);
+      turn(ra), turn(rb);
+    }
   };
 
   // ---- epilogue: a token block (16 rows) of a wave at a time through its part of a weight stage, so that
