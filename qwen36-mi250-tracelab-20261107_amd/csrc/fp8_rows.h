@@ -16,8 +16,8 @@ namespace moe {
 constexpr float kE4m3Max = 448.0f;
 constexpr int kMostRows = (1 << 26) - 4;  // a launch has fewer than 2^32 threads, 64 a row
 
-__device__ __forceinline__ float row_scale(float amax) {
-  return amax > 0.f ? fmaxf(amax, 0x1p-100f) / kE4m3Max : 1.0f;
+__device__ __forceinline__ float row_scale(float amax, float least = 0x1p-100f) {
+  return amax > 0.f ? fmaxf(amax, least) / kE4m3Max : 1.0f;
 }
 // v, or NaN where v is not finite. A maximum with NaN is the other operand, so such values do not count
 // for an amax.

@@ -10,9 +10,11 @@
 namespace moe {
 namespace {
 
+constexpr float kFloatMax = 3.402823466e+38f;
+
 // Stores a row of HC chunks of 8 fp32 values per lane (at c * 512 + 8 lane), of which each stands for
-// `times` as much, as e4m3 with its scale.
-template <int HC>
+// `times` as much (TIMES: not 1, in [1, 2)), as e4m3 with its scale.
+template <int HC, bool TIMES>
 __device__ __forceinline__ void store_row8(float (&v)[HC][8], float times, int n, int lane,
                                            uint8_t* q, float* scale) {
   float amax = 0.f;
@@ -21,7 +23,18 @@ __device__ __forceinline__ void store_row8(float (&v)[HC][8], float times, int n
 #pragma unroll
     for (int j = 0; j < 8; ++j) amax = amax_with(amax, v[c][j]);
   amax = wave_max(amax);
-  const float s = row_scale(amax);
+  if (TIMES && amax * times > kFloatMax) {  // values that are infinite with it
+    amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < HC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (fabsf(v[c][j]) * times > kFloatMax) v[c][j] = __builtin_nanf("");
+        amax = amax_with(amax, v[c][j]);
+      }
+    amax = wave_max(amax);
+  }
+  const float s = TIMES ? row_scale(amax, 0x1p-100f / times) : row_scale(amax);
   const float r = 1.0f / s;
 #pragma unroll
   for (int c = 0; c < HC; ++c) {
@@ -51,7 +64,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint16_t* x, int T,
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[c][2 * j] = bf_lo(u[j]), v[c][2 * j + 1] = bf_hi(u[j]);
   }
-  store_row8<HC>(v, 1.0f, n, lane, q + row * n, scale + row);
+  store_row8<HC, false>(v, 1.0f, n, lane, q + row * n, scale + row);
 }
 
 // total and norm as k_add_rms. The 8-bit rows come from the fp32 norm t r (1 + w), of which only r's
@@ -101,7 +114,7 @@ __global__ __launch_bounds__(256) void k_add_rms_fp8(const uint16_t* x, const ui
     }
     store_row<HC>(norm + row * H, H, lane, wv);
   }
-  store_row8<HC>(v, rest, H, lane, q + row * H, scale + row);
+  store_row8<HC, true>(v, rest, H, lane, q + row * H, scale + row);
 }
 
 }  // namespace
