@@ -138,7 +138,8 @@ def add_rms_moe_fp8(x: torch.Tensor, h: torch.Tensor | None, norm_weight: torch.
     e4m3 rows for ``ops.experts_fp8`` and as bf16 for the router and the shared expert
     (``ops.linear``, its activation and product in the epilogues). Needs fp8 experts. Results
     differ from ``add_rms_moe``'s by the rounding of the activations to e4m3, before each of the two
-    products; the routing is the same."""
+    products. The routing is the same but for the last bit of a logit with up to 4 tokens, whose
+    router there sums in another order."""
     shape = x.shape
     x2 = _bf16_rows(x, "x")
     h2 = None if h is None else _bf16_rows(h, "h").reshape(x2.shape)

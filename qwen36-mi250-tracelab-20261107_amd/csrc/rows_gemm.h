@@ -232,7 +232,8 @@ __device__ __forceinline__ void rows_linear_store(const RowsGemm& a, long long m
       if (n + i < a.N) out[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
   }
 }
-// Their weight scales and biases (zeros past N).
+// Their weight scales and biases (zeros past N). The bias's type is tested at each value, so that a bf16 one
+// is eight loads of 2 bytes, one after the other.
 __device__ __forceinline__ void rows_linear_cols(const RowsGemm& a, int n, float (&ws)[8],
                                                  float (&bias)[8]) {
 #pragma unroll
@@ -289,8 +290,8 @@ __device__ __forceinline__ void rows_gate_up_cols(const RowsGemm& a, int e, int 
 
 // kRowsDown: outputs n .. n + 7 of pair row p, whose scales are ws, on their way to the weighted sum:
 // fp16 values of a power of two 2^ex per 32 columns, ex + 128 in a byte of its own, the largest
-// between 2^14 and 2^15. At bf16's size, its error (2^-12 of a value) does not show in the sum,
-// where bf16's (2^-9) was as large as the result's own rounding. The four lanes of 32 columns are
+// between 2^14 and 2^15. At bf16's size, its error (2^-11 of a value at most) does not show in the sum,
+// where bf16's (2^-8) was as large as the result's own rounding. The four lanes of 32 columns are
 // neighbours and all called; live: the row is stored.
 __device__ __forceinline__ void rows_down_out(const RowsGemm& a, bool live, long long p, int n,
                                               const float (&ws)[8], float (&v)[8]) {
