@@ -253,11 +253,12 @@ int moe_add_rmsnorm_fp8(const void* x, const void* h, const void* weight, int T,
 
 /* out [M, N] = bf16(residual + mul * act(x_scale_m w_scale_n sum_k x[m, k] w[n, k] + bias_n)),
  * fp32 in between; of more than 16 e4m3 rows the matrix instruction may cut each product, towards
- * zero, below 2^-13 of the largest of its eight neighbours along K. x [M, K] and w [N, K] are both
- * bf16 (no scales, K a multiple of 8) or both e4m3 (MOE_WEIGHTS_FP8_E4M3, with x_scale [M] and
- * w_scale [N], K a multiple of 16); rows are ldx / ldw elements (at most 4 MiB) apart and start at multiples of 16 bytes. bias [N] is bf16,
- * or fp32 with bias_f32; mul and residual are [M, N] bf16, 16-byte aligned as out. bias, mul and
- * residual may be null. */
+ * zero, below 2^-13 of the largest of its eight neighbours along K. The sum is multiplied by
+ * x_scale, then by w_scale, each in fp32 (infinite where it passes that on the way). x [M, K] and
+ * w [N, K] are both bf16 (no scales, K a multiple of 8) or both e4m3 (MOE_WEIGHTS_FP8_E4M3, with
+ * x_scale [M] and w_scale [N], K a multiple of 16); rows are ldx / ldw elements (at most 4 MiB)
+ * apart and start at multiples of 16 bytes. bias [N] is bf16, or fp32 with bias_f32; mul and
+ * residual are [M, N] bf16, 16-byte aligned as out. bias, mul and residual may be null. */
 #define MOE_ACT_NONE 0
 #define MOE_ACT_RELU 1
 #define MOE_ACT_SILU 2

@@ -524,8 +524,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, x_scale: torch.Tensor | None = N
     [N, K], fp32 up to the one rounding. Operands are both bf16 (K a multiple of 8) or both
     float8_e4m3fn with fp32 row scales ``x_scale`` [...] and ``w_scale`` [N] (K a multiple of
     16); of more than 16 e4m3 rows the matrix instruction may cut each product below 2^-13 of the largest of
-    its eight neighbours along K, which shows only where much larger products cancel. ``bias`` [N] is bf16 or fp32, ``mul`` and ``residual`` [..., N] bf16; ``activation`` is
-    None, "relu", "silu", "gelu" or "gelu_tanh". Rows of ``w`` may be strided, as in a slice of a
+    its eight neighbours along K, which shows only where much larger products cancel. Sums are scaled by
+    ``x_scale``, then by ``w_scale``, in fp32. ``bias`` [N] is bf16 or fp32, ``mul`` and ``residual``
+    [..., N] bf16; ``activation`` is None, "relu", "silu", "gelu" or "gelu_tanh". Rows of ``w`` may be strided, as in a slice of a
     packed weight, if each starts at a multiple of 16 bytes; rows of ``x`` that are not so are
     copied."""
     if not (x.is_cuda and w.is_cuda):
